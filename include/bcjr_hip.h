@@ -266,6 +266,107 @@ int bcjr_rht(const float* W, float* out, int64_t m, int64_t n, const float* sign
 int bcjr_rht_batched(const float* W, float* out, int64_t batch, int64_t m, int64_t n,
                      const float* sign_l, const float* sign_r, int inverse, hipStream_t stream);
 
+/* ---- Mixture-of-experts products, routing and distillation ----------------
+ *
+ * What a layer of quantized experts and its training loop do around the
+ * quantizer.  The reference leaves these to eager torch (its expert loop,
+ * src/qat/qat_moe_layer.py:85-116, and its KL-distillation drivers in src/qat).
+ * T tokens, E experts, k experts a token, M = T*k pairs sorted by expert. */
+
+/* Element types of the operands below. */
+enum { BCJR_F32 = 0, BCJR_BF16 = 1, BCJR_F16 = 2 };
+
+/* Bytes of workspace bcjr_moe_route wants (0 for a few tokens). */
+int bcjr_moe_route_workspace(int64_t T, int64_t E, size_t* bytes);
+
+/* Routing of T tokens to k of E experts (1 <= k <= min(E, 64), E <= 1024).
+ * logits (T, E) of `dtype`, row stride ld elements.  valid (T) bytes, or NULL
+ * for all: a token whose byte is 0 gets no expert.
+ *   experts (T, k)  the k largest logits of each token, in descending order,
+ *                   equal ones by the lowest index, NaN above all; -1 where
+ *                   fewer than k logits are above -inf
+ *   weights (T, k)  softmax of the logits at those experts or, with
+ *                   renormalize, the softmax over the chosen; 0 at -1
+ *   offsets (E+1)   first sorted place of each expert's pairs; [E] is their number
+ *   rows (T*k)      token of each sorted place (by expert, then token); -1 behind
+ *                   offsets[E]
+ *   slots (T, k)    sorted place of each pair; -1 for none
+ * ws: bcjr_moe_route_workspace bytes, or NULL where that is 0. */
+int bcjr_moe_route(const void* logits, int dtype, int64_t ld, const uint8_t* valid, int64_t T,
+                   int64_t E, int k, int renormalize, float* weights, int32_t* experts,
+                   int32_t* offsets, int32_t* rows, int32_t* slots, void* ws, size_t ws_bytes,
+                   hipStream_t stream);
+
+/* g_logits (T, E) of `dtype` from g_weights (T, k) and the outputs of
+ * bcjr_moe_route; the choice of experts has no gradient. */
+int bcjr_moe_route_backward(const void* logits, int dtype, int64_t ld, const uint8_t* valid,
+                            int64_t T, int64_t E, int k, int renormalize, const float* weights,
+                            const int32_t* experts, const float* g_weights, void* g_logits,
+                            hipStream_t stream);
+
+/* out (M, N) = a times each row's expert matrix.  Row p of a is row rows[p] of
+ * `a` (a_rows rows, row stride lda elements; a place outside [0, a_rows) is a
+ * zero row), or row p where rows is NULL.  Places [offsets[e], offsets[e+1])
+ * belong to expert e (offsets (E+1) on the device, ascending, offsets[0] taken as
+ * 0 and all clamped to [0, M]); the places behind offsets[E] get zeros.
+ *   b_is_nk = 1: b (E, N, K), out = a b^T (weights as a linear layer holds them)
+ *   b_is_nk = 0: b (E, K, N), out = a b
+ * BF16 or F16, products summed in float32.  E <= 1024; M < 2^31. */
+int bcjr_grouped_matmul(const void* a, int dtype, int64_t lda, int64_t a_rows,
+                        const int32_t* rows, const void* b, int b_is_nk, const int32_t* offsets,
+                        int64_t E, int64_t M, int64_t N, int64_t K, void* out,
+                        hipStream_t stream);
+
+/* out (E, N, K) = sum over each expert's places of a[p]^T b[p]: a (M, N), row
+ * stride lda; b (b_rows, K), row stride ldb, rows through `rows` as above.  An
+ * expert without places gets zeros.  out is float32 (out_f32) or of `dtype`. */
+int bcjr_grouped_wgrad(const void* a, int dtype, int64_t lda, const void* b, int64_t ldb,
+                       int64_t b_rows, const int32_t* rows, const int32_t* offsets, int64_t E,
+                       int64_t M, int64_t N, int64_t K, int out_f32, void* out,
+                       hipStream_t stream);
+
+/* out (T, N) = sum_j weights[t][j] y[slots[t][j]], y (M, N) of `dtype` with row
+ * stride ldy, summed in float32 in the order of j; weights (T, k), or NULL for
+ * ones; a slot outside [0, M) adds nothing. */
+int bcjr_moe_combine(const void* y, int dtype, int64_t ldy, const float* weights,
+                     const int32_t* slots, int64_t T, int k, int64_t M, int64_t N, void* out,
+                     hipStream_t stream);
+
+/* Gradients of bcjr_moe_combine: g_y (M, N) of `dtype` (rows[p] < 0: zeros) and
+ * g_weights (T, k), from g_out (T, N) with row stride ldg.  M = T*k. */
+int bcjr_moe_combine_backward(const void* y, int dtype, int64_t ldy, const float* weights,
+                              const int32_t* slots, const int32_t* rows, const void* g_out,
+                              int64_t ldg, int64_t T, int k, int64_t M, int64_t N, void* g_y,
+                              float* g_weights, hipStream_t stream);
+
+/* Divergence of a student from a teacher's top logits, row by row.  logits
+ * (T, V) of `dtype`, row stride ld; values, indices (T, K): the teacher's
+ * logits and their vocabulary entries, an index outside [0, V) for none;
+ * teacher_lse (T): log-sum-exp of the teacher's logits over temperature, or NULL.
+ *   q = exp(values / temperature - teacher_lse), or the softmax over the K
+ *   entries without it; p = softmax(logits / temperature);
+ *   loss = sum q (log q - log p) + r (log r - log p_r), r = 1 - sum q (0 if
+ *   under 1e-6 or without teacher_lse), p_r the student's mass outside the entries.
+ * A row without entries has the loss 0 and the gradient 0.  stats (T, 4) keeps
+ * what the backward needs, or NULL. */
+int bcjr_topk_distill(const void* logits, int dtype, int64_t ld, const float* values,
+                      const int32_t* indices, const float* teacher_lse, float temperature,
+                      int64_t T, int64_t V, int64_t K, float* loss, float* stats,
+                      hipStream_t stream);
+
+/* g_logits (T, V) = g_loss[t] d loss[t] / d logits, from the stats of
+ * bcjr_topk_distill.  A row whose g_loss is 0 gets zeros. */
+int bcjr_topk_distill_backward(const void* logits, int dtype, int64_t ld, const float* values,
+                               const int32_t* indices, float temperature, int64_t T, int64_t V,
+                               int64_t K, const float* stats, const float* g_loss,
+                               void* g_logits, hipStream_t stream);
+
+/* Loss and gradient in one launch, where g_loss is known beforehand. */
+int bcjr_topk_distill_both(const void* logits, int dtype, int64_t ld, const float* values,
+                           const int32_t* indices, const float* teacher_lse, float temperature,
+                           int64_t T, int64_t V, int64_t K, const float* g_loss, float* loss,
+                           void* g_logits, hipStream_t stream);
+
 /* Static name of a status code. */
 const char* bcjr_strerror(int status);
 

@@ -26,6 +26,8 @@ from .rht import (  # noqa: F401
     make_sign_vector,
 )
 from .experts import bcjr_quantize_experts, quantize_moe_experts, ste_quantize_experts  # noqa: F401
+from .moe import MoERoute, grouped_matmul, moe_combine, moe_route  # noqa: F401
+from .distill import topk_distill_loss, topk_distill_loss_and_grad  # noqa: F401
 from .ste import (  # noqa: F401
     TrellisQuantSTE, TrellisQuantSTE_IP, ptq_residual, quantize_forward_gpu, quantize_forward_gpu_no_rht,
     measure_ptq_residual, quantize_forward_numpy, replay_walks,

@@ -26,6 +26,9 @@ BCJR_OK, BCJR_EINVAL, BCJR_EUNSUPPORTED, BCJR_EWORKSPACE, BCJR_EHIP = 0, -1, -2,
 EXPORTS = (
     "bcjr_workspace_bytes", "bcjr_forward", "bcjr_forward_noalloc", "bcjr_forward_internals", "bcjr_forward_entropy", "bcjr_backward",
     "bcjr_viterbi", "bcjr_viterbi_constrained", "bcjr_viterbi_trace", "bcjr_decode", "bcjr_dequant", "bcjr_codebook", "bcjr_hadamard", "bcjr_rht", "bcjr_rht_batched",
+    "bcjr_moe_route_workspace", "bcjr_moe_route", "bcjr_moe_route_backward", "bcjr_grouped_matmul",
+    "bcjr_grouped_wgrad", "bcjr_moe_combine", "bcjr_moe_combine_backward", "bcjr_topk_distill",
+    "bcjr_topk_distill_backward", "bcjr_topk_distill_both",
     "bcjr_strerror", "bcjr_last_error", "bcjr_version",
 )
 
@@ -115,9 +118,23 @@ def load(path: str = LIB_PATH):
     lib.bcjr_rht.argtypes = [vp, vp, i64, i64, vp, vp, i32, vp]
     lib.bcjr_rht_batched.argtypes = [vp, vp, i64, i64, i64, vp, vp, i32, vp]
     lib.bcjr_dequant.argtypes = [pp, vp, i32, vp, vp, i64, i64, i32, i32, ctypes.c_double, vp, vp]
+    f32 = ctypes.c_float
+    lib.bcjr_moe_route_workspace.argtypes = [i64, i64, ctypes.POINTER(sz)]
+    lib.bcjr_moe_route.argtypes = [vp, i32, i64, vp, i64, i64, i32, i32, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.bcjr_moe_route_backward.argtypes = [vp, i32, i64, vp, i64, i64, i32, i32, vp, vp, vp, vp, vp]
+    lib.bcjr_grouped_matmul.argtypes = [vp, i32, i64, i64, vp, vp, i32, vp, i64, i64, i64, i64, vp, vp]
+    lib.bcjr_grouped_wgrad.argtypes = [vp, i32, i64, vp, i64, i64, vp, vp, i64, i64, i64, i64, i32, vp, vp]
+    lib.bcjr_moe_combine.argtypes = [vp, i32, i64, vp, vp, i64, i32, i64, i64, vp, vp]
+    lib.bcjr_moe_combine_backward.argtypes = [vp, i32, i64, vp, vp, vp, vp, i64, i64, i32, i64, i64, vp, vp, vp]
+    lib.bcjr_topk_distill.argtypes = [vp, i32, i64, vp, vp, vp, f32, i64, i64, i64, vp, vp, vp]
+    lib.bcjr_topk_distill_backward.argtypes = [vp, i32, i64, vp, vp, f32, i64, i64, i64, vp, vp, vp, vp]
+    lib.bcjr_topk_distill_both.argtypes = [vp, i32, i64, vp, vp, vp, f32, i64, i64, i64, vp, vp, vp, vp]
     lib.bcjr_strerror.argtypes = [i32]
     for name in ("bcjr_workspace_bytes", "bcjr_forward", "bcjr_forward_noalloc", "bcjr_forward_internals", "bcjr_forward_entropy",
-                 "bcjr_backward", "bcjr_viterbi", "bcjr_viterbi_constrained", "bcjr_viterbi_trace", "bcjr_decode", "bcjr_dequant", "bcjr_codebook", "bcjr_hadamard", "bcjr_rht", "bcjr_rht_batched"):
+                 "bcjr_backward", "bcjr_viterbi", "bcjr_viterbi_constrained", "bcjr_viterbi_trace", "bcjr_decode", "bcjr_dequant", "bcjr_codebook", "bcjr_hadamard", "bcjr_rht", "bcjr_rht_batched",
+                 "bcjr_moe_route_workspace", "bcjr_moe_route", "bcjr_moe_route_backward", "bcjr_grouped_matmul",
+                 "bcjr_grouped_wgrad", "bcjr_moe_combine", "bcjr_moe_combine_backward", "bcjr_topk_distill",
+                 "bcjr_topk_distill_backward", "bcjr_topk_distill_both"):
         getattr(lib, name).restype = i32
     for name in ("bcjr_strerror", "bcjr_last_error", "bcjr_version"):
         getattr(lib, name).restype = ctypes.c_char_p

@@ -35,6 +35,14 @@ int hip_fail(hipError_t e, const char* what) {
   return fail(BCJR_EHIP, "%s: %s", what, hipGetErrorString(e));
 }
 
+}  // namespace
+
+namespace bcjr {
+int report_failure(int status, const char* text) { return fail(status, "%s", text); }
+}  // namespace bcjr
+
+namespace {
+
 struct DeviceInfo {
   bool valid = false;
   int num_cu = 0;

@@ -1,0 +1,75 @@
+// Device helpers shared by the mixture-of-experts and distillation kernels:
+// element types, 16-byte vectors, wave and workgroup reductions.
+#pragma once
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace bcjr {
+
+// Element types by the ids of the C ABI (BCJR_F32, BCJR_BF16, BCJR_F16).  The
+// 16-bit types are held as their bits; all arithmetic is float32.
+struct F32 {
+  using raw = float;
+  static __device__ __forceinline__ float get(raw x) { return x; }
+  static __device__ __forceinline__ raw put(float x) { return x; }
+};
+struct BF16 {
+  using raw = uint16_t;
+  static __device__ __forceinline__ float get(raw x) { return __uint_as_float((uint32_t)x << 16); }
+  static __device__ __forceinline__ raw put(float x) {  // to nearest, ties to even
+    return __builtin_bit_cast(uint16_t, (__bf16)x);
+  }
+};
+struct F16 {
+  using raw = uint16_t;
+  static __device__ __forceinline__ float get(raw x) { return (float)__builtin_bit_cast(_Float16, x); }
+  static __device__ __forceinline__ raw put(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+};
+
+// 16 bytes of elements: 4 of float32, 8 of the 16-bit types.
+template <class E>
+struct alignas(16) Vec16 {
+  static constexpr int N = 16 / sizeof(typename E::raw);
+  typename E::raw v[N];
+};
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+  return x;
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
+// Sum and maximum over a workgroup of NW waves; every thread gets the result.
+// `part` holds NW floats and may be reused after the next barrier.
+template <int NW>
+__device__ __forceinline__ float group_sum(float x, float* part) {
+  x = wave_sum(x);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) s += part[i];
+  return s;
+}
+
+template <int NW>
+__device__ __forceinline__ float group_max(float x, float* part) {
+  x = wave_max(x);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+  __syncthreads();
+  float s = part[0];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) s = fmaxf(s, part[i]);
+  return s;
+}
+
+}  // namespace bcjr

@@ -26,31 +26,12 @@
 // Codebook resolution (recognising a plain table as 1MAD / 3INST / HYB) and the
 // autograd formulas stay in the Python package; these operators take the
 // resolved code, its LUT or table, and L, k, V, Q.
-#include <ATen/ATen.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/core/DeviceGuard.h>
-#include <torch/library.h>
+#include "bcjr_torch.h"
 
 #include <optional>
 #include <tuple>
 
-#include "../../include/bcjr_hip.h"
-
 namespace {
-
-using at::Tensor;
-
-// A failed C ABI call: a RuntimeError whose message starts with "bcjr status
-// <n>:" (the Python package re-raises it as BcjrError with that status).
-void check(int status, const char* what) {
-  if (status != BCJR_OK)
-    TORCH_CHECK(false, "bcjr status ", status, ": ", what, " failed: ", bcjr_strerror(status), ": ",
-                bcjr_last_error());
-}
-
-hipStream_t stream_of(const Tensor& t) {
-  return at::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
-}
 
 bcjr_problem problem(int64_t L, int64_t k, int64_t V, int64_t B, int64_t N, int64_t code, int64_t Q,
                      bool t_per_seq) {
@@ -67,10 +48,6 @@ bcjr_problem problem(int64_t L, int64_t k, int64_t V, int64_t B, int64_t N, int6
 }
 
 const float* fptr(const std::optional<Tensor>& t) { return t ? t->data_ptr<float>() : nullptr; }
-
-void same_device(const Tensor& ref, const std::optional<Tensor>& t, const char* name) {
-  if (t) TORCH_CHECK(t->device() == ref.device(), name, " is on ", t->device(), " but the launch runs on ", ref.device());
-}
 
 Tensor as_f32(const Tensor& t) { return t.to(at::kFloat).contiguous(); }
 
