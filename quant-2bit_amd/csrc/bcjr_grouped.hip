@@ -200,9 +200,302 @@ __global__ __launch_bounds__(256) void wgrad_any_kernel(GroupedParams P) {
       }
 }
 
+// --------------------------------------------------- rows in 16-byte chunks
+//
+// BM x BN outputs per workgroup of eight waves, 64 of the reduction at a time:
+// global loads of the next 64 go to registers while the matrix instructions
+// work from one of two LDS buffers, and are written to the other behind them.
+//
+// An operand whose reduction runs along its rows (K tiles) lies in LDS as
+// [row][64] and is read 16 bytes a lane; one whose reduction runs across its
+// rows (the weights of the rows' gradient, both sides of the weights' gradient)
+// as [64][column], read with the transposing LDS read: 16 lanes take a 4 x 16
+// block, each ends with one column's four values.  The 16-byte chunks of a row
+// are permuted by its number so that the 16 lanes of a read's pass meet
+// distinct banks.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kBK = 64;
+constexpr int kFastThreads = 512;
+
+__device__ const u32x4 kZeros = {0, 0, 0, 0};  // what lanes outside an operand load
+
+// Row tile: byte offset of 16-byte chunk c (of 8) of row r.
+__device__ __forceinline__ int row_at(int r, int c) { return r * 128 + ((c ^ ((r >> 1) & 7)) << 4); }
+// Column tile of width W: byte offset of 16-byte chunk c of reduction row r.
+template <int W>
+__device__ __forceinline__ int col_at(int r, int c) {
+  return r * W * 2 + ((c ^ (2 * ((r & 3) | ((r >> 1) & 4)))) << 4);
+}
+
+// Fragment of 16 outputs (from o on) x 32 of the reduction (step ks of 2).
+template <bool COL, int W>
+__device__ __forceinline__ u16x8 fragment(const char* lds, int o, int ks) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+  if constexpr (!COL) {
+    return *(const u16x8*)(lds + row_at(o + i, 4 * ks + g));
+  } else {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const int r = 32 * ks + 8 * g + (i >> 2);
+    const char* p = lds + col_at<W>(r, (o >> 3) + ((i >> 1) & 1)) + (i & 1) * 8;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * W * 2));
+    return __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+}
+
+// One thread's share of an operand's tile: N chunks of 16 bytes.
+template <int ROWS, bool COL>
+struct Stage {
+  static constexpr int kChunks = ROWS * 8 / kFastThreads;
+  u32x4 v[kChunks];
+};
+
+enum { GM_NK, GM_KN, GM_WG };  // w (E, N, K); w (E, K, N); the weights' gradient
+
+struct Place {
+  int e;
+  int64_t r0, r1;  // rows of the tile (products), of the group (weights' gradient)
+  int64_t n0;
+};
+
+// The workgroup's output tile of a product.  Workgroups go to the chip's eight
+// dies in turn, each with an L2 of its own, so each die takes a contiguous part
+// of the tiles, ordered by expert, then column, then row: an expert's weights
+// are read by one die (two at the seams), and neighbours share a column panel.
+template <int BM>
+__device__ __forceinline__ bool find_place(const int32_t* offsets, int E, int64_t M, int nt, int64_t id, Place* out) {
+  const int lane = threadIdx.x & 63;
+  auto group = [&](int e, int64_t* a, int64_t* b) {
+    *a = *b = 0;
+    if (e <= E) {
+      *a = e == 0 ? 0 : min((int64_t)max(offsets[e], 0), M);
+      *b = e == E ? M : min((int64_t)max(offsets[e + 1], 0), M);
+      *b = max(*a, *b);
+    }
+    return (int)((*b - *a + BM - 1) / BM);
+  };
+  int64_t total = 0;
+  for (int i = 0; i <= E; i += 64) {
+    int64_t a, b;
+    int n = group(i + lane, &a, &b);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o);
+    total += n;
+  }
+  total *= nt;
+  const int64_t per = (total + 7) / 8, at = (id & 7) * per + (id >> 3);
+  if ((id >> 3) >= per || at >= total) return false;
+  int64_t done = 0;
+  for (int i = 0; i <= E; i += 64) {
+    int64_t a, b;
+    const int n = group(i + lane, &a, &b);
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(upto, o);
+      if (lane >= o) upto += y;
+    }
+    const int64_t first = (done + upto - n) * nt;
+    const unsigned long long here = __ballot(at >= first && at < first + (int64_t)n * nt);
+    if (here) {
+      const int src = __ffsll(here) - 1;
+      const int ea = __shfl((int)a, src), eb = __shfl((int)b, src), en = __shfl(n, src);
+      const int64_t f = (done + __shfl(upto - n, src)) * nt;
+      const int local = (int)(at - f);
+      out->e = i + src;
+      out->r0 = ea + (int64_t)(local % en) * BM;
+      out->r1 = min(out->r0 + BM, (int64_t)eb);
+      out->n0 = local / en;
+      return true;
+    }
+    done += __shfl(upto, 63);
+  }
+  return false;
+}
+
+template <class E, class O, int MODE, int BM, int BN>
+__global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedParams P) {
+  constexpr bool ACOL = MODE == GM_WG, BCOL = MODE != GM_NK;
+  constexpr int WM = BM >= 128 ? 2 : 1, WN = 8 / WM;        // waves along rows and columns
+  constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;       // 16 x 16 blocks of a wave
+  constexpr int kABytes = BM * kBK * 2, kBytes = kABytes + BN * kBK * 2;
+  extern __shared__ __align__(16) char lds[];  // two buffers of kBytes
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+
+  Place t;
+  int64_t K;  // the reduction's length
+  if constexpr (MODE == GM_WG) {
+    const int64_t tm = (P.N + BM - 1) / BM, tn = (P.K + BN - 1) / BN, total = tm * tn * P.E;
+    const int64_t per = (total + 7) / 8, at = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= per || at >= total) return;
+    t.e = (int)(at / (tm * tn));
+    t.r0 = t.e == 0 ? 0 : min((int64_t)max(P.offsets[t.e], 0), P.M);
+    t.r1 = max(t.r0, min((int64_t)max(P.offsets[t.e + 1], 0), P.M));
+    t.n0 = at % (tm * tn);
+    K = t.r1 - t.r0;
+  } else {
+    if (!find_place<BM>(P.offsets, P.E, P.M, (int)((P.N + BN - 1) / BN), blockIdx.x, &t)) return;
+    K = t.e == P.E ? 0 : P.K;
+  }
+  // m0: first row (product) or column of dy (weights' gradient); n0: first column
+  const int64_t m0 = MODE == GM_WG ? t.n0 / ((P.K + BN - 1) / BN) * BM : t.r0;
+  const int64_t n0 = (MODE == GM_WG ? t.n0 % ((P.K + BN - 1) / BN) : t.n0) * BN;
+  const int64_t mend = MODE == GM_WG ? P.N : t.r1, nend = MODE == GM_WG ? P.K : P.N;
+
+  // global addresses of this thread's chunks
+  constexpr int SA = BM * 8 / kFastThreads, SB = BN * 8 / kFastThreads;
+  const uint16_t* ap[SA];
+  const uint16_t* bp[SB];
+  int64_t alim[SA], blim[SB];  // the chunk exists while k0 is below
+  const uint16_t* a = (const uint16_t*)P.a;
+  const uint16_t* b = (const uint16_t*)P.b;
+  if constexpr (MODE != GM_WG) b += (int64_t)t.e * P.N * P.K;
+#pragma unroll
+  for (int s = 0; s < SA; ++s) {
+    const int q = tid + kFastThreads * s;
+    if constexpr (!ACOL) {
+      const int64_t p = m0 + (q >> 3);
+      int64_t r = -1;
+      if (p < mend) r = P.rows ? P.rows[p] : p;
+      const bool ok = r >= 0 && r < P.a_rows;
+      ap[s] = a + (ok ? r * P.lda : 0) + (q & 7) * 8;
+      alim[s] = ok ? K - (q & 7) * 8 : 0;
+    } else {
+      const int r = q / (BM / 8), c = q % (BM / 8);
+      ap[s] = a + (t.r0 + r) * P.lda + m0 + c * 8;
+      alim[s] = m0 + c * 8 < mend ? K - r : 0;
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < SB; ++s) {
+    const int q = tid + kFastThreads * s;
+    if constexpr (!BCOL) {
+      const int64_t n = n0 + (q >> 3);
+      bp[s] = b + (n < nend ? n : 0) * P.K + (q & 7) * 8;
+      blim[s] = n < nend ? K - (q & 7) * 8 : 0;
+    } else {
+      const int r = q / (BN / 8), c = q % (BN / 8);
+      bp[s] = b + (MODE == GM_WG ? 0 : r * P.N) + n0 + c * 8;
+      blim[s] = n0 + c * 8 < nend ? K - r : 0;
+    }
+  }
+  u32x4 av[SA], bv[SB];
+  auto load = [&](int64_t k0) {
+#pragma unroll
+    for (int s = 0; s < SA; ++s) {
+      const uint16_t* p = ap[s] + (ACOL ? k0 * P.lda : k0);
+      av[s] = *(const u32x4*)(k0 < alim[s] ? p : (const uint16_t*)&kZeros);
+    }
+#pragma unroll
+    for (int s = 0; s < SB; ++s) {
+      const uint16_t* p;
+      bool ok = k0 < blim[s];
+      if constexpr (MODE == GM_WG) {
+        int64_t r = t.r0 + k0 + (tid + kFastThreads * s) / (BN / 8);
+        if (P.rows && ok) r = P.rows[r];
+        ok = ok && r >= 0 && r < P.b_rows;
+        p = bp[s] + (ok ? r * P.ldb : 0);
+      } else {
+        p = bp[s] + (BCOL ? k0 * P.N : k0);
+      }
+      bv[s] = *(const u32x4*)(ok ? p : (const uint16_t*)&kZeros);
+    }
+  };
+  auto store = [&](char* to) {
+#pragma unroll
+    for (int s = 0; s < SA; ++s) {
+      const int q = tid + kFastThreads * s;
+      const int at = ACOL ? col_at<BM>(q / (BM / 8), q % (BM / 8)) : row_at(q >> 3, q & 7);
+      *(u32x4*)(to + at) = av[s];
+    }
+#pragma unroll
+    for (int s = 0; s < SB; ++s) {
+      const int q = tid + kFastThreads * s;
+      const int at = BCOL ? col_at<BN>(q / (BN / 8), q % (BN / 8)) : row_at(q >> 3, q & 7);
+      *(u32x4*)(to + kABytes + at) = bv[s];
+    }
+  };
+
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  const bool busy = m0 + wm < mend && n0 + wn < nend;  // whole waves
+  f32x4 acc[MI][NJ] = {};
+  const int64_t steps = (K + kBK - 1) / kBK;
+  if (steps) {
+    load(0);
+    store(lds);
+    if (steps > 1) load(kBK);
+    __syncthreads();
+  }
+  for (int64_t it = 0; it < steps; ++it) {
+    const char* from = lds + (it & 1) * kBytes;
+    if (busy) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        u16x8 fa[MI], fb[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) fb[j] = fragment<BCOL, BN>(from + kABytes, wn + 16 * j, ks);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[i] = fragment<ACOL, BM>(from, wm + 16 * i, ks);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[i][j] = mfma16<E>(fb[j], fa[i], acc[i][j]);
+      }
+    }
+    if (it + 1 < steps) {
+      store(lds + ((it + 1) & 1) * kBytes);
+      if (it + 2 < steps) load((it + 2) * kBK);
+      __syncthreads();
+    }
+  }
+  if (!busy) return;
+
+  // lane: row (lane & 15), four neighbouring columns
+  typename O::raw* out = (typename O::raw*)P.out + (MODE == GM_WG ? (int64_t)t.e * P.N * P.K : 0);
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int64_t m = m0 + wm + 16 * i + (lane & 15);
+    if (m >= mend) continue;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int64_t n = n0 + wn + 16 * j + 4 * (lane >> 4);
+      if (n >= nend) continue;
+      struct alignas(4 * sizeof(typename O::raw)) { typename O::raw v[4]; } r;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) r.v[c] = O::put(acc[i][j][c]);
+      *(decltype(r)*)(out + m * nend + n) = r;
+    }
+  }
+}
+
+template <class E, class O, int MODE, int BM, int BN>
+hipError_t launch_tile(const GroupedParams& P, hipStream_t stream) {
+  const void* fn = (const void*)grouped_tile_kernel<E, O, MODE, BM, BN>;
+  constexpr int bytes = 2 * (BM + BN) * kBK * 2;
+  hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return e;
+  int64_t tiles = MODE == GM_WG ? (P.N + BM - 1) / BM * ((P.K + BN - 1) / BN) * P.E
+                                : max_tiles(P.M, P.E, BM) * ((P.N + BN - 1) / BN);
+  tiles = (tiles + 7) / 8 * 8;
+  void* args[] = {(void*)&P};
+  return hipLaunchKernel(fn, dim3((unsigned)tiles), dim3(kFastThreads), args, bytes, stream);
+}
+
+// 16-byte chunks: aligned bases, and row lengths and strides of whole chunks.
+bool chunked(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
+
 }  // namespace
 
 hipError_t launch_grouped(const GroupedParams& P, int dtype, bool b_is_nk, hipStream_t stream) {
+  if (P.K % 8 == 0 && P.N % 8 == 0 && chunked(P.a, P.lda) && chunked(P.b, 8) && chunked(P.out, 8)) {
+    if (dtype == 1)
+      return b_is_nk ? launch_tile<BF16, BF16, GM_NK, 256, 256>(P, stream)
+                     : launch_tile<BF16, BF16, GM_KN, 256, 256>(P, stream);
+    return b_is_nk ? launch_tile<F16, F16, GM_NK, 256, 256>(P, stream)
+                   : launch_tile<F16, F16, GM_KN, 256, 256>(P, stream);
+  }
   const void* fn = dtype == 1 ? (b_is_nk ? (const void*)grouped_any_kernel<BF16, true>
                                          : (const void*)grouped_any_kernel<BF16, false>)
                               : (b_is_nk ? (const void*)grouped_any_kernel<F16, true>
@@ -213,6 +506,13 @@ hipError_t launch_grouped(const GroupedParams& P, int dtype, bool b_is_nk, hipSt
 }
 
 hipError_t launch_grouped_wgrad(const GroupedParams& P, int dtype, bool out_f32, hipStream_t stream) {
+  if (P.K % 8 == 0 && P.N % 8 == 0 && chunked(P.a, P.lda) && chunked(P.b, P.ldb) && chunked(P.out, 8)) {
+    if (dtype == 1)
+      return out_f32 ? launch_tile<BF16, F32, GM_WG, 256, 256>(P, stream)
+                     : launch_tile<BF16, BF16, GM_WG, 256, 256>(P, stream);
+    return out_f32 ? launch_tile<F16, F32, GM_WG, 256, 256>(P, stream)
+                   : launch_tile<F16, F16, GM_WG, 256, 256>(P, stream);
+  }
   const void* fn = dtype == 1 ? (out_f32 ? (const void*)wgrad_any_kernel<BF16, F32>
                                          : (const void*)wgrad_any_kernel<BF16, BF16>)
                               : (out_f32 ? (const void*)wgrad_any_kernel<F16, F32>
