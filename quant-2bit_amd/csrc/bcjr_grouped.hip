@@ -203,8 +203,9 @@ __global__ __launch_bounds__(256) void wgrad_any_kernel(GroupedParams P) {
 // --------------------------------------------------- rows in 16-byte chunks
 //
 // BM x BN outputs per workgroup of eight waves, 64 of the reduction at a time:
-// global loads of the next 64 go to registers while the matrix instructions
-// work from one of two LDS buffers, and are written to the other behind them.
+// loads straight into LDS fill one of two buffers while the matrix instructions
+// work from the other.  Lanes outside an operand read past the buffer
+// descriptor's end, which gives zeros.
 //
 // An operand whose reduction runs along its rows (K tiles) lies in LDS as
 // [row][64] and is read 16 bytes a lane; one whose reduction runs across its
@@ -218,8 +219,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBK = 64;
 constexpr int kFastThreads = 512;
-
-__device__ const u32x4 kZeros = {0, 0, 0, 0};  // what lanes outside an operand load
 
 // Row tile: byte offset of 16-byte chunk c (of 8) of row r.
 __device__ __forceinline__ int row_at(int r, int c) { return r * 128 + ((c ^ ((r >> 1) & 7)) << 4); }
@@ -245,13 +244,6 @@ __device__ __forceinline__ u16x8 fragment(const char* lds, int o, int ks) {
   }
 }
 
-// One thread's share of an operand's tile: N chunks of 16 bytes.
-template <int ROWS, bool COL>
-struct Stage {
-  static constexpr int kChunks = ROWS * 8 / kFastThreads;
-  u32x4 v[kChunks];
-};
-
 enum { GM_NK, GM_KN, GM_WG };  // w (E, N, K); w (E, K, N); the weights' gradient
 
 struct Place {
@@ -264,6 +256,12 @@ struct Place {
 // dies in turn, each with an L2 of its own, so each die takes a contiguous part
 // of the tiles, ordered by expert, then column, then row: an expert's weights
 // are read by one die (two at the seams), and neighbours share a column panel.
+// A value that all lanes have alike, in scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)x) | (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
+}
+
 template <int BM>
 __device__ __forceinline__ bool find_place(const int32_t* offsets, int E, int64_t M, int nt, int64_t id, Place* out) {
   const int lane = threadIdx.x & 63;
@@ -301,19 +299,24 @@ __device__ __forceinline__ bool find_place(const int32_t* offsets, int E, int64_
     const unsigned long long here = __ballot(at >= first && at < first + (int64_t)n * nt);
     if (here) {
       const int src = __ffsll(here) - 1;
-      const int ea = __shfl((int)a, src), eb = __shfl((int)b, src), en = __shfl(n, src);
-      const int64_t f = (done + __shfl(upto - n, src)) * nt;
-      const int local = (int)(at - f);
-      out->e = i + src;
+      const int ea = uniform(__shfl((int)a, src)), eb = uniform(__shfl((int)b, src)), en = uniform(__shfl(n, src));
+      const int64_t f = (uniform((int)done) + uniform(__shfl(upto - n, src))) * (int64_t)nt;
+      const int local = uniform((int)(at - f));
+      out->e = uniform(i + src);
       out->r0 = ea + (int64_t)(local % en) * BM;
-      out->r1 = min(out->r0 + BM, (int64_t)eb);
-      out->n0 = local / en;
+      out->r0 = uniform(out->r0);
+      out->r1 = uniform(min(out->r0 + BM, (int64_t)eb));
+      out->n0 = uniform(local / en);
       return true;
     }
     done += __shfl(upto, 63);
   }
   return false;
 }
+
+typedef __attribute__((address_space(3))) void lds_void;
+constexpr int kAhead = 2;  // groups of matrix instructions that a fragment is read ahead
+constexpr uint32_t kOutside = 0xffffffffu;  // a buffer offset that loads zeros
 
 template <class E, class O, int MODE, int BM, int BN>
 __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedParams P) {
@@ -322,10 +325,10 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
   constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;       // 16 x 16 blocks of a wave
   constexpr int kABytes = BM * kBK * 2, kBytes = kABytes + BN * kBK * 2;
   extern __shared__ __align__(16) char lds[];  // two buffers of kBytes
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   Place t;
-  int64_t K;  // the reduction's length
+  int K;  // the reduction's length
   if constexpr (MODE == GM_WG) {
     const int64_t tm = (P.N + BM - 1) / BM, tn = (P.K + BN - 1) / BN, total = tm * tn * P.E;
     const int64_t per = (total + 7) / 8, at = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
@@ -334,122 +337,144 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
     t.r0 = t.e == 0 ? 0 : min((int64_t)max(P.offsets[t.e], 0), P.M);
     t.r1 = max(t.r0, min((int64_t)max(P.offsets[t.e + 1], 0), P.M));
     t.n0 = at % (tm * tn);
-    K = t.r1 - t.r0;
+    t.r0 = uniform(t.r0);
+    t.r1 = uniform(t.r1);
+    K = (int)(t.r1 - t.r0);
   } else {
     if (!find_place<BM>(P.offsets, P.E, P.M, (int)((P.N + BN - 1) / BN), blockIdx.x, &t)) return;
-    K = t.e == P.E ? 0 : P.K;
+    K = t.e == P.E ? 0 : (int)P.K;
   }
   // m0: first row (product) or column of dy (weights' gradient); n0: first column
   const int64_t m0 = MODE == GM_WG ? t.n0 / ((P.K + BN - 1) / BN) * BM : t.r0;
   const int64_t n0 = (MODE == GM_WG ? t.n0 % ((P.K + BN - 1) / BN) : t.n0) * BN;
   const int64_t mend = MODE == GM_WG ? P.N : t.r1, nend = MODE == GM_WG ? P.K : P.N;
 
-  // global addresses of this thread's chunks
-  constexpr int SA = BM * 8 / kFastThreads, SB = BN * 8 / kFastThreads;
-  const uint16_t* ap[SA];
-  const uint16_t* bp[SB];
-  int64_t alim[SA], blim[SB];  // the chunk exists while k0 is below
-  const uint16_t* a = (const uint16_t*)P.a;
-  const uint16_t* b = (const uint16_t*)P.b;
-  if constexpr (MODE != GM_WG) b += (int64_t)t.e * P.N * P.K;
-#pragma unroll
-  for (int s = 0; s < SA; ++s) {
-    const int q = tid + kFastThreads * s;
-    if constexpr (!ACOL) {
-      const int64_t p = m0 + (q >> 3);
-      int64_t r = -1;
-      if (p < mend) r = P.rows ? P.rows[p] : p;
-      const bool ok = r >= 0 && r < P.a_rows;
-      ap[s] = a + (ok ? r * P.lda : 0) + (q & 7) * 8;
-      alim[s] = ok ? K - (q & 7) * 8 : 0;
-    } else {
-      const int r = q / (BM / 8), c = q % (BM / 8);
-      ap[s] = a + (t.r0 + r) * P.lda + m0 + c * 8;
-      alim[s] = m0 + c * 8 < mend ? K - r : 0;
-    }
-  }
-#pragma unroll
-  for (int s = 0; s < SB; ++s) {
-    const int q = tid + kFastThreads * s;
-    if constexpr (!BCOL) {
-      const int64_t n = n0 + (q >> 3);
-      bp[s] = b + (n < nend ? n : 0) * P.K + (q & 7) * 8;
-      blim[s] = n < nend ? K - (q & 7) * 8 : 0;
-    } else {
-      const int r = q / (BN / 8), c = q % (BN / 8);
-      bp[s] = b + (MODE == GM_WG ? 0 : r * P.N) + n0 + c * 8;
-      blim[s] = n0 + c * 8 < nend ? K - r : 0;
-    }
-  }
-  u32x4 av[SA], bv[SB];
-  auto load = [&](int64_t k0) {
+  // Buffer s of a wave is 1 KiB of LDS: 8 rows of a row tile, 2 or 4 of a column
+  // tile, wave by wave.  This thread's row, chunk and byte offset in the operand
+  // (kOutside: none).
+  constexpr int SA = BM * kBK * 2 / 8192, SB = BN * kBK * 2 / 8192;
+  constexpr int AR = ACOL ? 512 / BM : 8, BR = BCOL ? 512 / BN : 8;  // rows of a KiB
+  auto row_of = [&](int s, int per) { return (s * 8 + wave) * per + lane / (64 / per); };
+  auto chunk_of = [&](int r, int per, bool col) {
+    const int pos = lane % (64 / per);
+    return col ? pos ^ (2 * ((r & 3) | ((r >> 1) & 4))) : pos ^ ((r >> 1) & 7);
+  };
+  const char* abase = (const char*)P.a;
+  const char* bbase = (const char*)P.b;
+  if constexpr (MODE != GM_WG) bbase += (int64_t)t.e * P.N * P.K * 2;
+  uint32_t aoff[SA], boff[SB];
+  if constexpr (!ACOL) {
+    if (!P.rows) abase += m0 * P.lda * 2;
 #pragma unroll
     for (int s = 0; s < SA; ++s) {
-      const uint16_t* p = ap[s] + (ACOL ? k0 * P.lda : k0);
-      av[s] = *(const u32x4*)(k0 < alim[s] ? p : (const uint16_t*)&kZeros);
+      const int r = row_of(s, AR);
+      aoff[s] = kOutside;
+      if (m0 + r < mend) {
+        const int64_t x = P.rows ? P.rows[m0 + r] : r;
+        if (!P.rows || (x >= 0 && x < P.a_rows)) aoff[s] = (uint32_t)((x * P.lda + chunk_of(r, AR, false) * 8) * 2);
+      }
     }
+  } else {
+    abase += (t.r0 * P.lda + m0) * 2;
+#pragma unroll
+    for (int s = 0; s < SA; ++s) {
+      const int r = row_of(s, AR), c = chunk_of(r, AR, true) * 8;
+      aoff[s] = m0 + c < mend ? (uint32_t)((r * P.lda + c) * 2) : kOutside;
+    }
+  }
+  if constexpr (!BCOL) {
+    bbase += n0 * P.K * 2;
 #pragma unroll
     for (int s = 0; s < SB; ++s) {
-      const uint16_t* p;
-      bool ok = k0 < blim[s];
-      if constexpr (MODE == GM_WG) {
-        int64_t r = t.r0 + k0 + (tid + kFastThreads * s) / (BN / 8);
-        if (P.rows && ok) r = P.rows[r];
-        ok = ok && r >= 0 && r < P.b_rows;
-        p = bp[s] + (ok ? r * P.ldb : 0);
-      } else {
-        p = bp[s] + (BCOL ? k0 * P.N : k0);
-      }
-      bv[s] = *(const u32x4*)(ok ? p : (const uint16_t*)&kZeros);
+      const int r = row_of(s, BR);
+      boff[s] = n0 + r < nend ? (uint32_t)((r * P.K + chunk_of(r, BR, false) * 8) * 2) : kOutside;
+    }
+  } else {
+    bbase += n0 * 2;
+    const int64_t ld = MODE == GM_WG ? P.ldb : P.N;
+    if (MODE == GM_WG && !P.rows) bbase += t.r0 * ld * 2;
+#pragma unroll
+    for (int s = 0; s < SB; ++s) {
+      const int r = row_of(s, BR), c = chunk_of(r, BR, true) * 8;
+      boff[s] = n0 + c < nend ? (uint32_t)(((MODE == GM_WG && P.rows ? 0 : r * ld) + c) * 2) : kOutside;
+    }
+  }
+  // the gathered rows of the weights' gradient, known one step ahead
+  int brow[SB];
+  auto find_rows = [&](int k0) {
+    if (!P.rows) return;
+#pragma unroll
+    for (int s = 0; s < SB; ++s) {
+      const int r = k0 + row_of(s, BR);
+      brow[s] = r < K ? P.rows[t.r0 + r] : -1;
     }
   };
-  auto store = [&](char* to) {
-#pragma unroll
-    for (int s = 0; s < SA; ++s) {
-      const int q = tid + kFastThreads * s;
-      const int at = ACOL ? col_at<BM>(q / (BM / 8), q % (BM / 8)) : row_at(q >> 3, q & 7);
-      *(u32x4*)(to + at) = av[s];
+  // rows or chunks that a step's reduction still has
+  const int acut = ACOL ? row_of(0, AR) : chunk_of(row_of(0, AR), AR, false) * 8;
+  const int bcut = BCOL ? row_of(0, BR) : chunk_of(row_of(0, BR), BR, false) * 8;
+  const bool gather = MODE == GM_WG && P.rows;
+  // chunk s of a step's SA + SB to its place in buffer `to`
+  auto load_one = [&](int s, int k0, char* to) {
+    if (s < SA) {
+      const auto ra = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)uniform((int64_t)(abase + (ACOL ? k0 * P.lda : (int64_t)k0) * 2)), 0, 0xfffffff0u, 0x00027000);
+      const uint32_t off = k0 + acut + (ACOL ? s * 8 * AR : 0) < K ? aoff[s] : kOutside;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)(to + (s * 8 + wave) * 1024), 16, off, 0, 0, 0);
+    } else {
+      const int b = s - SA;
+      const int64_t adv = gather ? 0 : BCOL ? k0 * (MODE == GM_WG ? P.ldb : P.N) : (int64_t)k0;
+      const auto rb = __builtin_amdgcn_make_buffer_rsrc((void*)uniform((int64_t)(bbase + adv * 2)), 0, 0xfffffff0u,
+                                                        0x00027000);
+      uint32_t off = k0 + bcut + (BCOL ? b * 8 * BR : 0) < K ? boff[b] : kOutside;
+      if (gather)
+        off = off != kOutside && brow[b] >= 0 && brow[b] < P.b_rows ? off + (uint32_t)(brow[b] * P.ldb * 2) : kOutside;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)(to + kABytes + (b * 8 + wave) * 1024), 16, off, 0, 0, 0);
     }
+  };
+  auto load = [&](int k0, char* to) {
 #pragma unroll
-    for (int s = 0; s < SB; ++s) {
-      const int q = tid + kFastThreads * s;
-      const int at = BCOL ? col_at<BN>(q / (BN / 8), q % (BN / 8)) : row_at(q >> 3, q & 7);
-      *(u32x4*)(to + kABytes + at) = bv[s];
-    }
+    for (int s = 0; s < SA + SB; ++s) load_one(s, k0, to);
+    if constexpr (MODE == GM_WG) find_rows(k0 + kBK);
   };
 
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const bool busy = m0 + wm < mend && n0 + wn < nend;  // whole waves
   f32x4 acc[MI][NJ] = {};
-  const int64_t steps = (K + kBK - 1) / kBK;
+  const int steps = (K + kBK - 1) / kBK;
   if (steps) {
-    load(0);
-    store(lds);
-    if (steps > 1) load(kBK);
+    if constexpr (MODE == GM_WG) find_rows(0);
+    load(0, lds);
+  }
+  for (int it = 0; it < steps; ++it) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this step's tiles are in LDS
     __syncthreads();
-  }
-  for (int64_t it = 0; it < steps; ++it) {
+    // past the end: zeros, where nothing is read
+    load((it + 1) * kBK, lds + (~it & 1) * kBytes);
+    if (!busy) continue;
     const char* from = lds + (it & 1) * kBytes;
-    if (busy) {
+    // MI groups of NJ matrix instructions for either half of the step; a group's
+    // fragments are read kAhead groups before it
+    u16x8 fa[kAhead + 1], fb[2][NJ];
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        u16x8 fa[MI], fb[NJ];
+    for (int j = 0; j < NJ; ++j) fb[0][j] = fragment<BCOL, BN>(from + kABytes, wn + 16 * j, 0);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) fb[j] = fragment<BCOL, BN>(from + kABytes, wn + 16 * j, ks);
+    for (int i = 0; i < kAhead; ++i) fa[i] = fragment<ACOL, BM>(from, wm + 16 * (i % MI), i / MI);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) fa[i] = fragment<ACOL, BM>(from, wm + 16 * i, ks);
+    for (int i = 0; i < 2 * MI; ++i) {
+      const int n = i + kAhead;
+      if (n < 2 * MI) fa[n % (kAhead + 1)] = fragment<ACOL, BM>(from, wm + 16 * (n % MI), n / MI);
+      if (i < MI) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) acc[i][j] = mfma16<E>(fb[j], fa[i], acc[i][j]);
+        for (int j = 0; j < NJ; ++j)
+          if (j * MI / NJ == i) fb[1][j] = fragment<BCOL, BN>(from + kABytes, wn + 16 * j, 1);
       }
-    }
-    if (it + 1 < steps) {
-      store(lds + ((it + 1) & 1) * kBytes);
-      if (it + 2 < steps) load((it + 2) * kBK);
-      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i % MI][j] = mfma16<E>(fb[i / MI][j], fa[i % (kAhead + 1)], acc[i % MI][j]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // no load is under way into LDS that the next workgroup owns
   if (!busy) return;
 
   // lane: row (lane & 15), four neighbouring columns
@@ -483,13 +508,18 @@ hipError_t launch_tile(const GroupedParams& P, hipStream_t stream) {
   return hipLaunchKernel(fn, dim3((unsigned)tiles), dim3(kFastThreads), args, bytes, stream);
 }
 
-// 16-byte chunks: aligned bases, and row lengths and strides of whole chunks.
-bool chunked(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
+// Rows in 16-byte chunks (an aligned base, a stride of whole chunks), within the
+// 32-bit offsets of a buffer descriptor: of the whole operand where rows are
+// gathered, else of the rows that a workgroup reads at a time.
+bool chunked(const void* p, int64_t ld, int64_t rows) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && rows * ld * 2 < (int64_t)0xfffffff0;
+}
 
 }  // namespace
 
 hipError_t launch_grouped(const GroupedParams& P, int dtype, bool b_is_nk, hipStream_t stream) {
-  if (P.K % 8 == 0 && P.N % 8 == 0 && chunked(P.a, P.lda) && chunked(P.b, 8) && chunked(P.out, 8)) {
+  if (P.K % 8 == 0 && P.N % 8 == 0 && chunked(P.a, P.lda, P.rows ? P.a_rows : 256) && chunked(P.b, 8, 1) &&
+      chunked(P.out, 8, 1)) {
     if (dtype == 1)
       return b_is_nk ? launch_tile<BF16, BF16, GM_NK, 256, 256>(P, stream)
                      : launch_tile<BF16, BF16, GM_KN, 256, 256>(P, stream);
@@ -506,7 +536,8 @@ hipError_t launch_grouped(const GroupedParams& P, int dtype, bool b_is_nk, hipSt
 }
 
 hipError_t launch_grouped_wgrad(const GroupedParams& P, int dtype, bool out_f32, hipStream_t stream) {
-  if (P.K % 8 == 0 && P.N % 8 == 0 && chunked(P.a, P.lda) && chunked(P.b, P.ldb) && chunked(P.out, 8)) {
+  if (P.K % 8 == 0 && P.N % 8 == 0 && chunked(P.a, P.lda, kBK) && chunked(P.b, P.ldb, P.rows ? P.b_rows : kBK) &&
+      chunked(P.out, 8, 1)) {
     if (dtype == 1)
       return out_f32 ? launch_tile<BF16, F32, GM_WG, 256, 256>(P, stream)
                      : launch_tile<BF16, BF16, GM_WG, 256, 256>(P, stream);
