@@ -252,43 +252,61 @@ struct Place {
   int64_t n0;
 };
 
-// The workgroup's output tile of a product.  Workgroups go to the chip's eight
-// dies in turn, each with an L2 of its own, so each die takes a contiguous part
-// of the tiles, ordered by expert, then column, then row: an expert's weights
-// are read by one die (two at the seams), and neighbours share a column panel.
 // A value that all lanes have alike, in scalar registers.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int64_t uniform(int64_t x) {
   return (int64_t)((uint64_t)(uint32_t)uniform((int)x) | (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
 }
 
+// Rows [a, b) of group e (E: those behind the last group; beyond: none).
+__device__ __forceinline__ void group_rows(const int32_t* offsets, int E, int M, int e, int* a, int* b) {
+  *a = *b = 0;
+  if (e <= E) {
+    *a = e == 0 ? 0 : min(max(offsets[e], 0), M);
+    *b = max(*a, e == E ? M : min(max(offsets[e + 1], 0), M));
+  }
+}
+
+// The workgroup's output tile of a product.  Workgroups go to the chip's eight
+// dies in turn, each with an L2 of its own, so each die takes a contiguous part
+// of the tiles, ordered by expert, then column, then row: an expert's weights
+// are read by one die (two at the seams), and neighbours share a column panel.
+// Tiles of full height come first, those with fewer rows after them, so that the
+// short ones fill the chip's last round.
 template <int BM>
-__device__ __forceinline__ bool find_place(const int32_t* offsets, int E, int64_t M, int nt, int64_t id, Place* out) {
+__device__ __forceinline__ bool find_place(const int32_t* offsets, int E, int M, int nt, int64_t id, Place* out) {
   const int lane = threadIdx.x & 63;
-  auto group = [&](int e, int64_t* a, int64_t* b) {
-    *a = *b = 0;
-    if (e <= E) {
-      *a = e == 0 ? 0 : min((int64_t)max(offsets[e], 0), M);
-      *b = e == E ? M : min((int64_t)max(offsets[e + 1], 0), M);
-      *b = max(*a, *b);
-    }
-    return (int)((*b - *a + BM - 1) / BM);
-  };
-  int64_t total = 0;
+  int64_t full = 0, part = 0;
   for (int i = 0; i <= E; i += 64) {
-    int64_t a, b;
-    int n = group(i + lane, &a, &b);
+    int a, b;
+    group_rows(offsets, E, M, i + lane, &a, &b);
+    int n = (b - a) / BM, m = (b - a) % BM != 0;
 #pragma unroll
     for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o);
-    total += n;
+    full += n;
+    part += __popcll(__ballot(m));
   }
-  total *= nt;
-  const int64_t per = (total + 7) / 8, at = (id & 7) * per + (id >> 3);
-  if ((id >> 3) >= per || at >= total) return false;
+  full = uniform(full) * nt;
+  part = uniform(part) * nt;
+  const int die = (int)(id & 7);
+  const int64_t per_full = (full + 7) / 8, per_part = (part + 7) / 8;
+  int64_t seq = id >> 3;
+  // how many of each this die has
+  const int64_t f0 = min(die * per_full, full), f1 = min(f0 + per_full, full);
+  const int64_t p0 = min(die * per_part, part), p1 = min(p0 + per_part, part);
+  const bool is_full = seq < f1 - f0;
+  int64_t at;
+  if (is_full) {
+    at = f0 + seq;
+  } else {
+    at = p0 + seq - (f1 - f0);
+    if (at >= p1) return false;
+  }
   int64_t done = 0;
   for (int i = 0; i <= E; i += 64) {
-    int64_t a, b;
-    const int n = group(i + lane, &a, &b);
+    int a, b;
+    group_rows(offsets, E, M, i + lane, &a, &b);
+    const int n = is_full ? (b - a) / BM : (b - a) % BM != 0;
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -299,14 +317,13 @@ __device__ __forceinline__ bool find_place(const int32_t* offsets, int E, int64_
     const unsigned long long here = __ballot(at >= first && at < first + (int64_t)n * nt);
     if (here) {
       const int src = __ffsll(here) - 1;
-      const int ea = uniform(__shfl((int)a, src)), eb = uniform(__shfl((int)b, src)), en = uniform(__shfl(n, src));
-      const int64_t f = (uniform((int)done) + uniform(__shfl(upto - n, src))) * (int64_t)nt;
+      const int ea = uniform(__shfl(a, src)), eb = uniform(__shfl(b, src)), en = uniform(__shfl(n, src));
+      const int64_t f = uniform((done + __shfl(upto - n, src)) * nt);
       const int local = uniform((int)(at - f));
       out->e = uniform(i + src);
-      out->r0 = ea + (int64_t)(local % en) * BM;
-      out->r0 = uniform(out->r0);
-      out->r1 = uniform(min(out->r0 + BM, (int64_t)eb));
-      out->n0 = uniform(local / en);
+      out->r0 = is_full ? ea + (int64_t)(local % en) * BM : ea + (int64_t)((eb - ea) / BM) * BM;
+      out->r1 = is_full ? out->r0 + BM : eb;
+      out->n0 = local / en;
       return true;
     }
     done += __shfl(upto, 63);
@@ -314,9 +331,58 @@ __device__ __forceinline__ bool find_place(const int32_t* offsets, int E, int64_
   return false;
 }
 
-typedef __attribute__((address_space(3))) void lds_void;
+// The workgroup's expert and output tile of the weights' gradient.  The tiles of
+// every expert are spread over all dies, xa x xb of them (xa xb = 8) across its
+// rows and columns, so that a die reads 1/xa of dy and 1/xb of x, and the dies
+// have alike to do however the rows are shared; the groups with the most rows
+// come first (up to 64 experts), so that the last to end are short.
+__device__ __forceinline__ bool find_wgrad_place(const GroupedParams& P, int tm, int tn, int64_t id, Place* out) {
+  const int lane = threadIdx.x & 63, die = (int)(id & 7);
+  const int xa = P.split, xb = 8 / xa;
+  const int pm = (tm + xa - 1) / xa, pn = (tn + xb - 1) / xb;
+  const int64_t seq = id >> 3;
+  int e = (int)(seq / (pm * pn));
+  const int local = (int)(seq % (pm * pn));
+  const int i = local / pn * xa + die / xb, j = local % pn * xb + die % xb;
+  if (e >= P.E || i >= tm || j >= tn) return false;
+  int a, b;
+  if (P.E <= 64) {
+    group_rows(P.offsets, P.E, (int)P.M, lane < P.E ? lane : P.E + 1, &a, &b);
+    const int n = b - a;
+    int rank = 0;
+    for (int o = 0; o < P.E; ++o) {
+      const int other = __builtin_amdgcn_readlane(n, o);
+      rank += other > n || (other == n && o < lane);
+    }
+    e = __ffsll(__ballot(lane < P.E && rank == e)) - 1;
+  }
+  group_rows(P.offsets, P.E, (int)P.M, e, &a, &b);
+  out->e = uniform(e);
+  out->r0 = uniform(a);
+  out->r1 = uniform(b);
+  out->n0 = (int64_t)i * tn + j;
+  return true;
+}
+
+typedef __attribute__((address_space(3))) char lds_char;
 constexpr int kAhead = 2;  // groups of matrix instructions that a fragment is read ahead
 constexpr uint32_t kOutside = 0xffffffffu;  // a buffer offset that loads zeros
+
+// Loads 16 bytes a lane from `base` + off into the KiB of LDS at `to` (uniform),
+// in lane order; no register receives data.  Written as an instruction because
+// the compiler lets the transposing LDS reads of the other buffer wait for every
+// such load that it sees.  Whoever reads the KiB waits for vmcnt first.
+__device__ __forceinline__ void load_to_lds(const char* base, uint32_t off, char* to) {
+  const uint64_t b = (uint64_t)uniform((int64_t)base);
+  const u32x4 desc = {(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, 0xfffffff0u, 0x00027000u};
+  const uint32_t at = (uint32_t)uniform((int)(uint32_t)(uintptr_t)(lds_char*)to);
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds"
+      ::"s"(at), "v"(off), "s"(desc)
+      : "memory", "m0");
+}
 
 template <class E, class O, int MODE, int BM, int BN>
 __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedParams P) {
@@ -330,18 +396,10 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
   Place t;
   int K;  // the reduction's length
   if constexpr (MODE == GM_WG) {
-    const int64_t tm = (P.N + BM - 1) / BM, tn = (P.K + BN - 1) / BN, total = tm * tn * P.E;
-    const int64_t per = (total + 7) / 8, at = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= per || at >= total) return;
-    t.e = (int)(at / (tm * tn));
-    t.r0 = t.e == 0 ? 0 : min((int64_t)max(P.offsets[t.e], 0), P.M);
-    t.r1 = max(t.r0, min((int64_t)max(P.offsets[t.e + 1], 0), P.M));
-    t.n0 = at % (tm * tn);
-    t.r0 = uniform(t.r0);
-    t.r1 = uniform(t.r1);
+    if (!find_wgrad_place(P, (int)((P.N + BM - 1) / BM), (int)((P.K + BN - 1) / BN), blockIdx.x, &t)) return;
     K = (int)(t.r1 - t.r0);
   } else {
-    if (!find_place<BM>(P.offsets, P.E, P.M, (int)((P.N + BN - 1) / BN), blockIdx.x, &t)) return;
+    if (!find_place<BM>(P.offsets, P.E, (int)P.M, (int)((P.N + BN - 1) / BN), blockIdx.x, &t)) return;
     K = t.e == P.E ? 0 : (int)P.K;
   }
   // m0: first row (product) or column of dy (weights' gradient); n0: first column
@@ -400,40 +458,33 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
     }
   }
   // the gathered rows of the weights' gradient, known one step ahead
-  int brow[SB];
+  uint32_t brow[SB];
+  const uint32_t bmost = (uint32_t)min(P.b_rows, (int64_t)INT32_MAX);
   auto find_rows = [&](int k0) {
     if (!P.rows) return;
 #pragma unroll
     for (int s = 0; s < SB; ++s) {
-      const int r = k0 + row_of(s, BR);
-      brow[s] = r < K ? P.rows[t.r0 + r] : -1;
+      const int r = min(k0 + row_of(s, BR), K - 1);  // rows past the end are not loaded
+      brow[s] = (uint32_t)P.rows[t.r0 + r];
     }
   };
   // rows or chunks that a step's reduction still has
   const int acut = ACOL ? row_of(0, AR) : chunk_of(row_of(0, AR), AR, false) * 8;
   const int bcut = BCOL ? row_of(0, BR) : chunk_of(row_of(0, BR), BR, false) * 8;
   const bool gather = MODE == GM_WG && P.rows;
-  // chunk s of a step's SA + SB to its place in buffer `to`
-  auto load_one = [&](int s, int k0, char* to) {
-    if (s < SA) {
-      const auto ra = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)uniform((int64_t)(abase + (ACOL ? k0 * P.lda : (int64_t)k0) * 2)), 0, 0xfffffff0u, 0x00027000);
-      const uint32_t off = k0 + acut + (ACOL ? s * 8 * AR : 0) < K ? aoff[s] : kOutside;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)(to + (s * 8 + wave) * 1024), 16, off, 0, 0, 0);
-    } else {
-      const int b = s - SA;
-      const int64_t adv = gather ? 0 : BCOL ? k0 * (MODE == GM_WG ? P.ldb : P.N) : (int64_t)k0;
-      const auto rb = __builtin_amdgcn_make_buffer_rsrc((void*)uniform((int64_t)(bbase + adv * 2)), 0, 0xfffffff0u,
-                                                        0x00027000);
-      uint32_t off = k0 + bcut + (BCOL ? b * 8 * BR : 0) < K ? boff[b] : kOutside;
-      if (gather)
-        off = off != kOutside && brow[b] >= 0 && brow[b] < P.b_rows ? off + (uint32_t)(brow[b] * P.ldb * 2) : kOutside;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)(to + kABytes + (b * 8 + wave) * 1024), 16, off, 0, 0, 0);
-    }
-  };
   auto load = [&](int k0, char* to) {
+    const char* pa = abase + (ACOL ? k0 * P.lda : (int64_t)k0) * 2;
+    const char* pb = bbase + (gather ? 0 : BCOL ? k0 * (MODE == GM_WG ? P.ldb : P.N) : (int64_t)k0) * 2;
 #pragma unroll
-    for (int s = 0; s < SA + SB; ++s) load_one(s, k0, to);
+    for (int s = 0; s < SA; ++s)
+      load_to_lds(pa, k0 + acut + (ACOL ? s * 8 * AR : 0) < K ? aoff[s] : kOutside, to + (s * 8 + wave) * 1024);
+#pragma unroll
+    for (int s = 0; s < SB; ++s) {
+      uint32_t off = k0 + bcut + (BCOL ? s * 8 * BR : 0) < K ? boff[s] : kOutside;
+      if constexpr (MODE == GM_WG)
+        if (gather) off = off != kOutside && brow[s] < bmost ? off + brow[s] * (uint32_t)(P.ldb * 2) : kOutside;
+      load_to_lds(pb, off, to + kABytes + (s * 8 + wave) * 1024);
+    }
     if constexpr (MODE == GM_WG) find_rows(k0 + kBK);
   };
 
@@ -501,10 +552,23 @@ hipError_t launch_tile(const GroupedParams& P, hipStream_t stream) {
   constexpr int bytes = 2 * (BM + BN) * kBK * 2;
   hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != hipSuccess) return e;
-  int64_t tiles = MODE == GM_WG ? (P.N + BM - 1) / BM * ((P.K + BN - 1) / BN) * P.E
-                                : max_tiles(P.M, P.E, BM) * ((P.N + BN - 1) / BN);
-  tiles = (tiles + 7) / 8 * 8;
-  void* args[] = {(void*)&P};
+  int64_t tiles;
+  GroupedParams Q = P;
+  if (MODE == GM_WG) {
+    const int64_t tm = (P.N + BM - 1) / BM, tn = (P.K + BN - 1) / BN;
+    // the split over the dies that leaves the fewest without a tile, of those the squarest
+    int64_t best = INT64_MAX;
+    for (int xa : {2, 4, 1, 8}) {
+      const int64_t per = (tm + xa - 1) / xa * ((tn + 8 / xa - 1) / (8 / xa));
+      if (per < best) best = per, Q.split = xa;
+    }
+    tiles = best * 8 * P.E;
+  } else {
+    // full and short tiles are each shared by the dies in equal parts
+    tiles = (max_tiles(P.M, P.E, BM) * ((P.N + BN - 1) / BN) + 7) / 8 * 8 + 8;
+  }
+  if (tiles > INT32_MAX) return hipErrorInvalidConfiguration;
+  void* args[] = {(void*)&Q};
   return hipLaunchKernel(fn, dim3((unsigned)tiles), dim3(kFastThreads), args, bytes, stream);
 }
 

@@ -80,6 +80,7 @@ struct GroupedParams {
   int64_t lda, ldb, a_rows, b_rows;
   int64_t M, N, K;
   int E;
+  int split;  // set by the launch
 };
 
 struct DistillParams {
