@@ -311,18 +311,31 @@ int bcjr_moe_route_backward(const void* logits, int dtype, int64_t ld, const uin
  * 0 and all clamped to [0, M]); the places behind offsets[E] get zeros.
  *   b_is_nk = 1: b (E, N, K), out = a b^T (weights as a linear layer holds them)
  *   b_is_nk = 0: b (E, K, N), out = a b
- * BF16 or F16, products summed in float32.  E <= 1024; M < 2^31. */
+ * with row stride ldb, the matrices of b back to back.
+ * BF16 or F16, products summed in float32.  E <= 1024; M < 2^31.
+ * Rows in 16-byte chunks (16-byte aligned bases, strides and K, for b_is_nk = 0 N
+ * too, multiples of 8) take the fast kernel, others one that is many times
+ * slower.  zero_padded = 1 says that the rows of a and b lie 8 elements apart or a
+ * multiple, with zeros between their ends and the next multiple of 8 (as
+ * bcjr_pad_rows makes them): then K and N may be any for the fast kernel. */
 int bcjr_grouped_matmul(const void* a, int dtype, int64_t lda, int64_t a_rows,
-                        const int32_t* rows, const void* b, int b_is_nk, const int32_t* offsets,
-                        int64_t E, int64_t M, int64_t N, int64_t K, void* out,
-                        hipStream_t stream);
+                        const int32_t* rows, const void* b, int64_t ldb, int b_is_nk,
+                        const int32_t* offsets, int64_t E, int64_t M, int64_t N, int64_t K,
+                        int zero_padded, void* out, hipStream_t stream);
+
+/* Copies rows of n elements (dtype_in: F32 or `dtype`), ld apart, to rows ldo apart
+ * (a multiple of 8, at least n) of dtype BF16 or F16, with zeros behind them; out
+ * 16-byte aligned.  float32 is rounded to the nearest, ties to even. */
+int bcjr_pad_rows(const void* x, int dtype_in, int64_t ld, int64_t rows, int64_t n, int dtype,
+                  void* out, int64_t ldo, hipStream_t stream);
 
 /* out (E, N, K) = sum over each expert's places of a[p]^T b[p]: a (M, N), row
  * stride lda; b (b_rows, K), row stride ldb, rows through `rows` as above.  An
- * expert without places gets zeros.  out is float32 (out_f32) or of `dtype`. */
+ * expert without places gets zeros.  out is float32 (out_f32) or of `dtype`.
+ * zero_padded as above. */
 int bcjr_grouped_wgrad(const void* a, int dtype, int64_t lda, const void* b, int64_t ldb,
                        int64_t b_rows, const int32_t* rows, const int32_t* offsets, int64_t E,
-                       int64_t M, int64_t N, int64_t K, int out_f32, void* out,
+                       int64_t M, int64_t N, int64_t K, int zero_padded, int out_f32, void* out,
                        hipStream_t stream);
 
 /* out (T, N) = sum_j weights[t][j] y[slots[t][j]], y (M, N) of `dtype` with row

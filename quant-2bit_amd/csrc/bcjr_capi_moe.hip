@@ -51,6 +51,8 @@ size_t route_ws(int64_t T, int64_t E) {
 
 constexpr int64_t kMaxDim = 1 << 20;
 
+int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+
 int check_grouped(int dtype, int64_t E, int64_t M, int64_t N, int64_t K) {
   if (int rc = check_dtype(dtype)) return rc;
   if (dtype == BCJR_F32) return fail(BCJR_EUNSUPPORTED, "grouped products are built for bfloat16 and float16 operands");
@@ -139,33 +141,58 @@ int bcjr_moe_route_backward(const void* logits, int dtype, int64_t ld, const uin
 }
 
 int bcjr_grouped_matmul(const void* a, int dtype, int64_t lda, int64_t a_rows, const int32_t* rows, const void* b,
-                        int b_is_nk, const int32_t* offsets, int64_t E, int64_t M, int64_t N, int64_t K, void* out,
-                        hipStream_t stream) {
+                        int64_t ldb, int b_is_nk, const int32_t* offsets, int64_t E, int64_t M, int64_t N, int64_t K,
+                        int zero_padded, void* out, hipStream_t stream) {
   if (int rc = check_grouped(dtype, E, M, N, K)) return rc;
   if (a_rows < 0 || (!rows && a_rows < M))
     return fail(BCJR_EINVAL, "a has %lld rows for M=%lld", (ll)a_rows, (ll)M);
+  const int64_t across = b_is_nk ? K : N;
   if (a_rows > 1 && lda < K) return fail(BCJR_EINVAL, "row stride %lld is below K=%lld", (ll)lda, (ll)K);
+  if (ldb < across) return fail(BCJR_EINVAL, "row stride %lld of b is below %lld", (ll)ldb, (ll)across);
+  if (zero_padded && (ldb < up8(across) || (a_rows > 1 && lda < up8(K)) || ldb % 8 || lda % 8))
+    return fail(BCJR_EINVAL, "zero-padded rows: strides %lld, %lld do not hold K=%lld, N=%lld in eights", (ll)lda,
+                (ll)ldb, (ll)K, (ll)N);
   if (M == 0) return BCJR_OK;
   if ((!a && a_rows) || !b || !offsets || !out) return fail(BCJR_EINVAL, "a, b, offsets and out must be non-NULL");
   bcjr::GroupedParams P = {};
   P.a = a, P.b = b, P.rows = rows, P.offsets = offsets, P.out = out;
-  P.lda = lda, P.a_rows = a_rows, P.M = M, P.N = N, P.K = K, P.E = (int)E;
+  P.lda = lda, P.ldb = ldb, P.a_rows = a_rows, P.M = M, P.N = N, P.K = K, P.E = (int)E;
+  P.zero_padded = zero_padded != 0;
   return launched(bcjr::launch_grouped(P, dtype, b_is_nk != 0, stream), "bcjr_grouped_matmul launch");
 }
 
 int bcjr_grouped_wgrad(const void* a, int dtype, int64_t lda, const void* b, int64_t ldb, int64_t b_rows,
                        const int32_t* rows, const int32_t* offsets, int64_t E, int64_t M, int64_t N, int64_t K,
-                       int out_f32, void* out, hipStream_t stream) {
+                       int zero_padded, int out_f32, void* out, hipStream_t stream) {
   if (int rc = check_grouped(dtype, E, M, N, K)) return rc;
   if (b_rows < 0 || (!rows && b_rows < M)) return fail(BCJR_EINVAL, "b has %lld rows for M=%lld", (ll)b_rows, (ll)M);
   if (M > 1 && lda < N) return fail(BCJR_EINVAL, "row stride %lld is below N=%lld", (ll)lda, (ll)N);
   if (b_rows > 1 && ldb < K) return fail(BCJR_EINVAL, "row stride %lld is below K=%lld", (ll)ldb, (ll)K);
+  if (zero_padded && (lda < up8(N) || ldb < up8(K) || lda % 8 || ldb % 8))
+    return fail(BCJR_EINVAL, "zero-padded rows: strides %lld, %lld do not hold N=%lld, K=%lld in eights", (ll)lda,
+                (ll)ldb, (ll)N, (ll)K);
   if (!offsets || !out || (M && (!a || (!b && b_rows))))
     return fail(BCJR_EINVAL, "a, b, offsets and out must be non-NULL");
   bcjr::GroupedParams P = {};
   P.a = a, P.b = b, P.rows = rows, P.offsets = offsets, P.out = out;
   P.lda = lda, P.ldb = ldb, P.a_rows = M, P.b_rows = b_rows, P.M = M, P.N = N, P.K = K, P.E = (int)E;
+  P.zero_padded = zero_padded != 0;
   return launched(bcjr::launch_grouped_wgrad(P, dtype, out_f32 != 0, stream), "bcjr_grouped_wgrad launch");
+}
+
+int bcjr_pad_rows(const void* x, int dtype_in, int64_t ld, int64_t rows, int64_t n, int dtype, void* out, int64_t ldo,
+                  hipStream_t stream) {
+  if (int rc = check_dtype(dtype_in)) return rc;
+  if (int rc = check_dtype(dtype)) return rc;
+  if (dtype == BCJR_F32 || (dtype_in != BCJR_F32 && dtype_in != dtype))
+    return fail(BCJR_EUNSUPPORTED, "padded copies are built from float32 or the 16-bit type itself to that type");
+  if (rows < 0 || n < 0) return fail(BCJR_EINVAL, "rows=%lld, n=%lld must be >= 0", (ll)rows, (ll)n);
+  if (rows > 1 && ld < n) return fail(BCJR_EINVAL, "row stride %lld is below n=%lld", (ll)ld, (ll)n);
+  if (ldo < n || ldo % 8) return fail(BCJR_EINVAL, "ldo=%lld must be a multiple of 8, at least n=%lld", (ll)ldo, (ll)n);
+  if (rows == 0 || ldo == 0) return BCJR_OK;
+  if ((!x && n) || !out) return fail(BCJR_EINVAL, "x and out must be non-NULL");
+  if (reinterpret_cast<uintptr_t>(out) & 15) return fail(BCJR_EINVAL, "out must be 16-byte aligned");
+  return launched(bcjr::launch_pad_rows(x, dtype_in, ld, rows, n, dtype, out, ldo, stream), "bcjr_pad_rows launch");
 }
 
 int bcjr_moe_combine(const void* y, int dtype, int64_t ldy, const float* weights, const int32_t* slots, int64_t T,

@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256) void grouped_any_kernel(GroupedParams P) {
   }
   __syncthreads();
   const uint16_t* a = (const uint16_t*)P.a;
-  const uint16_t* b = (const uint16_t*)P.b + (int64_t)t.e * P.N * P.K;
+  const uint16_t* b = (const uint16_t*)P.b + (int64_t)t.e * (NK ? P.N : P.K) * P.ldb;
   f32x4 acc[2][2] = {};
   for (int64_t k0 = 0; k0 < P.K; k0 += kTk) {
     const int kc = (int)min((int64_t)kTk, P.K - k0);
@@ -136,10 +136,10 @@ __global__ __launch_bounds__(256) void grouped_any_kernel(GroupedParams P) {
       const int64_t r = row_of[m];
       As[m][k] = r >= 0 && k < kc ? a[r * P.lda + k0 + k] : (uint16_t)0;
       if (NK) {
-        Bs[m][k] = m < nc && k < kc ? b[(n0 + m) * P.K + k0 + k] : (uint16_t)0;
+        Bs[m][k] = m < nc && k < kc ? b[(n0 + m) * P.ldb + k0 + k] : (uint16_t)0;
       } else {
         const int n = i % kT, kk = i / kT;
-        Bs[n][kk] = n < nc && kk < kc ? b[(k0 + kk) * P.N + n0 + n] : (uint16_t)0;
+        Bs[n][kk] = n < nc && kk < kc ? b[(k0 + kk) * P.ldb + n0 + n] : (uint16_t)0;
       }
     }
     __syncthreads();
@@ -222,10 +222,15 @@ constexpr int kFastThreads = 512;
 
 // Row tile: byte offset of 16-byte chunk c (of 8) of row r.
 __device__ __forceinline__ int row_at(int r, int c) { return r * 128 + ((c ^ ((r >> 1) & 7)) << 4); }
-// Column tile of width W: byte offset of 16-byte chunk c of reduction row r.
+// Column tile of width W: permutation of reduction row r's chunks, and byte
+// offset of its chunk c.  (Rows of 64 columns are half of the banks.)
+template <int W>
+__device__ __forceinline__ int col_swizzle(int r) {
+  return W >= 128 ? 2 * ((r & 3) | ((r >> 1) & 4)) : 2 * (((r >> 1) & 1) | ((r >> 2) & 2));
+}
 template <int W>
 __device__ __forceinline__ int col_at(int r, int c) {
-  return r * W * 2 + ((c ^ (2 * ((r & 3) | ((r >> 1) & 4)))) << 4);
+  return r * W * 2 + ((c ^ col_swizzle<W>(r)) << 4);
 }
 
 // Fragment of 16 outputs (from o on) x 32 of the reduction (step ks of 2).
@@ -387,7 +392,8 @@ __device__ __forceinline__ void load_to_lds(const char* base, uint32_t off, char
 template <class E, class O, int MODE, int BM, int BN>
 __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedParams P) {
   constexpr bool ACOL = MODE == GM_WG, BCOL = MODE != GM_NK;
-  constexpr int WM = BM >= 128 ? 2 : 1, WN = 8 / WM;        // waves along rows and columns
+  constexpr int WM = 2, WN = 4;                             // waves along rows and columns
+  static_assert(BM % 64 == 0 && BN % 64 == 0);
   constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;       // 16 x 16 blocks of a wave
   constexpr int kABytes = BM * kBK * 2, kBytes = kABytes + BN * kBK * 2;
   extern __shared__ __align__(16) char lds[];  // two buffers of kBytes
@@ -413,13 +419,11 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
   constexpr int SA = BM * kBK * 2 / 8192, SB = BN * kBK * 2 / 8192;
   constexpr int AR = ACOL ? 512 / BM : 8, BR = BCOL ? 512 / BN : 8;  // rows of a KiB
   auto row_of = [&](int s, int per) { return (s * 8 + wave) * per + lane / (64 / per); };
-  auto chunk_of = [&](int r, int per, bool col) {
-    const int pos = lane % (64 / per);
-    return col ? pos ^ (2 * ((r & 3) | ((r >> 1) & 4))) : pos ^ ((r >> 1) & 7);
-  };
+  auto a_chunk = [&](int r) { return lane % (64 / AR) ^ (ACOL ? col_swizzle<BM>(r) : (r >> 1) & 7); };
+  auto b_chunk = [&](int r) { return lane % (64 / BR) ^ (BCOL ? col_swizzle<BN>(r) : (r >> 1) & 7); };
   const char* abase = (const char*)P.a;
   const char* bbase = (const char*)P.b;
-  if constexpr (MODE != GM_WG) bbase += (int64_t)t.e * P.N * P.K * 2;
+  if constexpr (MODE != GM_WG) bbase += (int64_t)t.e * (MODE == GM_NK ? P.N : P.K) * P.ldb * 2;
   uint32_t aoff[SA], boff[SB];
   if constexpr (!ACOL) {
     if (!P.rows) abase += m0 * P.lda * 2;
@@ -429,32 +433,31 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
       aoff[s] = kOutside;
       if (m0 + r < mend) {
         const int64_t x = P.rows ? P.rows[m0 + r] : r;
-        if (!P.rows || (x >= 0 && x < P.a_rows)) aoff[s] = (uint32_t)((x * P.lda + chunk_of(r, AR, false) * 8) * 2);
+        if (!P.rows || (x >= 0 && x < P.a_rows)) aoff[s] = (uint32_t)((x * P.lda + a_chunk(r) * 8) * 2);
       }
     }
   } else {
     abase += (t.r0 * P.lda + m0) * 2;
 #pragma unroll
     for (int s = 0; s < SA; ++s) {
-      const int r = row_of(s, AR), c = chunk_of(r, AR, true) * 8;
+      const int r = row_of(s, AR), c = a_chunk(r) * 8;
       aoff[s] = m0 + c < mend ? (uint32_t)((r * P.lda + c) * 2) : kOutside;
     }
   }
   if constexpr (!BCOL) {
-    bbase += n0 * P.K * 2;
+    bbase += n0 * P.ldb * 2;
 #pragma unroll
     for (int s = 0; s < SB; ++s) {
       const int r = row_of(s, BR);
-      boff[s] = n0 + r < nend ? (uint32_t)((r * P.K + chunk_of(r, BR, false) * 8) * 2) : kOutside;
+      boff[s] = n0 + r < nend ? (uint32_t)((r * P.ldb + b_chunk(r) * 8) * 2) : kOutside;
     }
   } else {
     bbase += n0 * 2;
-    const int64_t ld = MODE == GM_WG ? P.ldb : P.N;
-    if (MODE == GM_WG && !P.rows) bbase += t.r0 * ld * 2;
+    if (MODE == GM_WG && !P.rows) bbase += t.r0 * P.ldb * 2;
 #pragma unroll
     for (int s = 0; s < SB; ++s) {
-      const int r = row_of(s, BR), c = chunk_of(r, BR, true) * 8;
-      boff[s] = n0 + c < nend ? (uint32_t)(((MODE == GM_WG && P.rows ? 0 : r * ld) + c) * 2) : kOutside;
+      const int r = row_of(s, BR), c = b_chunk(r) * 8;
+      boff[s] = n0 + c < nend ? (uint32_t)(((MODE == GM_WG && P.rows ? 0 : r * P.ldb) + c) * 2) : kOutside;
     }
   }
   // the gathered rows of the weights' gradient, known one step ahead
@@ -469,12 +472,12 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
     }
   };
   // rows or chunks that a step's reduction still has
-  const int acut = ACOL ? row_of(0, AR) : chunk_of(row_of(0, AR), AR, false) * 8;
-  const int bcut = BCOL ? row_of(0, BR) : chunk_of(row_of(0, BR), BR, false) * 8;
+  const int acut = ACOL ? row_of(0, AR) : a_chunk(row_of(0, AR)) * 8;
+  const int bcut = BCOL ? row_of(0, BR) : b_chunk(row_of(0, BR)) * 8;
   const bool gather = MODE == GM_WG && P.rows;
   auto load = [&](int k0, char* to) {
     const char* pa = abase + (ACOL ? k0 * P.lda : (int64_t)k0) * 2;
-    const char* pb = bbase + (gather ? 0 : BCOL ? k0 * (MODE == GM_WG ? P.ldb : P.N) : (int64_t)k0) * 2;
+    const char* pb = bbase + (gather ? 0 : BCOL ? k0 * P.ldb : (int64_t)k0) * 2;
 #pragma unroll
     for (int s = 0; s < SA; ++s)
       load_to_lds(pa, k0 + acut + (ACOL ? s * 8 * AR : 0) < K ? aoff[s] : kOutside, to + (s * 8 + wave) * 1024);
@@ -530,6 +533,23 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
 
   // lane: row (lane & 15), four neighbouring columns
   typename O::raw* out = (typename O::raw*)P.out + (MODE == GM_WG ? (int64_t)t.e * P.N * P.K : 0);
+  if (nend % 4 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int64_t m = m0 + wm + 16 * i + (lane & 15);
+      if (m >= mend) continue;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int64_t n = n0 + wn + 16 * j + 4 * (lane >> 4);
+        if (n >= nend) continue;
+        struct alignas(4 * sizeof(typename O::raw)) { typename O::raw v[4]; } r;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) r.v[c] = O::put(acc[i][j][c]);
+        *(decltype(r)*)(out + m * nend + n) = r;
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int64_t m = m0 + wm + 16 * i + (lane & 15);
@@ -537,11 +557,9 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int64_t n = n0 + wn + 16 * j + 4 * (lane >> 4);
-      if (n >= nend) continue;
-      struct alignas(4 * sizeof(typename O::raw)) { typename O::raw v[4]; } r;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) r.v[c] = O::put(acc[i][j][c]);
-      *(decltype(r)*)(out + m * nend + n) = r;
+      for (int c = 0; c < 4; ++c)
+        if (n + c < nend) out[m * nend + n + c] = O::put(acc[i][j][c]);
     }
   }
 }
@@ -579,16 +597,48 @@ bool chunked(const void* p, int64_t ld, int64_t rows) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && rows * ld * 2 < (int64_t)0xfffffff0;
 }
 
+// Side of the square output tiles.  Larger tiles load less for the same work and
+// smaller ones leave fewer compute units idle; the counts below take every group
+// to have a short tile.  Measured (microseconds at 256 / 128 / 64, bfloat16):
+//   products  4096 tokens x 8, 64 experts, 2048 x 2048 (1,536 tiles of 256)  410 / 476 / -
+//             1024 x 8, 64, 2048 x 2048 (768)       178 / 178 / 215
+//             256 x 8, 64, 2048 x 2048 (576)        127 / 120 / -
+//             2048 x 4, 64, 1024 x 1024 (384)        53 /  40 /  54
+//             1024 x 2, 8, 1024 x 1024 (192 of 128)  34 /  16 /  19
+//             512 rows on 8, 512 x 512 (60 of 128)   22 /  10 /   7
+//   and of a few rows, where the weights' bytes count and not the row tiles:
+//             4 tokens x 8, 64, 2048 x 2048 (512 of 128)  34 / 26 / 26
+//             8 x 2, 8, 4096 x 4096 (256 of 128)          57 / 39 / 32
+//   weights' gradient  8 experts, 2048 x 2048 (512)    25 / 29 / 44
+//             16, 1024 x 1024 (256; 1,024 of 128)      22 / 21 / 31
+//             4, 512 x 2048 (256 of 128)               64 / 28 / 21
+int product_side(const GroupedParams& P) {
+  const int64_t groups = P.E < P.M ? P.E : P.M;
+  auto tiles = [&](int64_t s) { return (P.M / s + groups) * ((P.N + s - 1) / s); };
+  if (tiles(256) >= 700) return 256;
+  return tiles(128) < (P.M <= 64 * groups ? 512 : 176) ? 64 : 128;
+}
+int wgrad_side(const GroupedParams& P) {
+  auto tiles = [&](int64_t s) { return P.E * ((P.N + s - 1) / s) * ((P.K + s - 1) / s); };
+  return tiles(256) >= 384 ? 256 : tiles(128) >= 400 ? 128 : 64;
+}
+
+template <class E, int MODE, class O>
+hipError_t launch_side(const GroupedParams& P, hipStream_t stream) {
+  const int side = MODE == GM_WG ? wgrad_side(P) : product_side(P);
+  return side == 256   ? launch_tile<E, O, MODE, 256, 256>(P, stream)
+         : side == 128 ? launch_tile<E, O, MODE, 128, 128>(P, stream)
+                       : launch_tile<E, O, MODE, 64, 64>(P, stream);
+}
+
 }  // namespace
 
 hipError_t launch_grouped(const GroupedParams& P, int dtype, bool b_is_nk, hipStream_t stream) {
-  if (P.K % 8 == 0 && P.N % 8 == 0 && chunked(P.a, P.lda, P.rows ? P.a_rows : 256) && chunked(P.b, 8, 1) &&
-      chunked(P.out, 8, 1)) {
+  if ((P.zero_padded || (P.K % 8 == 0 && (b_is_nk || P.N % 8 == 0))) &&
+      chunked(P.a, P.lda, P.rows ? P.a_rows : 256) && chunked(P.b, P.ldb, 256)) {
     if (dtype == 1)
-      return b_is_nk ? launch_tile<BF16, BF16, GM_NK, 256, 256>(P, stream)
-                     : launch_tile<BF16, BF16, GM_KN, 256, 256>(P, stream);
-    return b_is_nk ? launch_tile<F16, F16, GM_NK, 256, 256>(P, stream)
-                   : launch_tile<F16, F16, GM_KN, 256, 256>(P, stream);
+      return b_is_nk ? launch_side<BF16, GM_NK, BF16>(P, stream) : launch_side<BF16, GM_KN, BF16>(P, stream);
+    return b_is_nk ? launch_side<F16, GM_NK, F16>(P, stream) : launch_side<F16, GM_KN, F16>(P, stream);
   }
   const void* fn = dtype == 1 ? (b_is_nk ? (const void*)grouped_any_kernel<BF16, true>
                                          : (const void*)grouped_any_kernel<BF16, false>)
@@ -600,13 +650,11 @@ hipError_t launch_grouped(const GroupedParams& P, int dtype, bool b_is_nk, hipSt
 }
 
 hipError_t launch_grouped_wgrad(const GroupedParams& P, int dtype, bool out_f32, hipStream_t stream) {
-  if (P.K % 8 == 0 && P.N % 8 == 0 && chunked(P.a, P.lda, kBK) && chunked(P.b, P.ldb, P.rows ? P.b_rows : kBK) &&
-      chunked(P.out, 8, 1)) {
+  if ((P.zero_padded || (P.K % 8 == 0 && P.N % 8 == 0)) && chunked(P.a, P.lda, kBK) &&
+      chunked(P.b, P.ldb, P.rows ? P.b_rows : kBK)) {
     if (dtype == 1)
-      return out_f32 ? launch_tile<BF16, F32, GM_WG, 256, 256>(P, stream)
-                     : launch_tile<BF16, BF16, GM_WG, 256, 256>(P, stream);
-    return out_f32 ? launch_tile<F16, F32, GM_WG, 256, 256>(P, stream)
-                   : launch_tile<F16, F16, GM_WG, 256, 256>(P, stream);
+      return out_f32 ? launch_side<BF16, GM_WG, F32>(P, stream) : launch_side<BF16, GM_WG, BF16>(P, stream);
+    return out_f32 ? launch_side<F16, GM_WG, F32>(P, stream) : launch_side<F16, GM_WG, F16>(P, stream);
   }
   const void* fn = dtype == 1 ? (out_f32 ? (const void*)wgrad_any_kernel<BF16, F32>
                                          : (const void*)wgrad_any_kernel<BF16, BF16>)
@@ -615,6 +663,49 @@ hipError_t launch_grouped_wgrad(const GroupedParams& P, int dtype, bool out_f32,
   void* args[] = {(void*)&P};
   return hipLaunchKernel(fn, dim3((unsigned)((P.N + kT - 1) / kT), (unsigned)((P.K + kT - 1) / kT), (unsigned)P.E),
                          dim3(256), args, 0, stream);
+}
+
+// ------------------------------------------------------------- padded copies
+
+// Rows of n elements, copied to rows of ldo with zeros behind them, float32
+// rounded to the 16-bit type.  A thread writes one 16-byte chunk, from loads that
+// need no alignment but the elements'.
+template <class E, class I>
+__global__ __launch_bounds__(256) void pad_rows_kernel(const typename I::raw* x, int64_t ld, int64_t rows, int64_t n,
+                                                       uint16_t* out, int64_t ldo) {
+  const int64_t per = ldo / 8, total = rows * per;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
+    const int64_t r = q / per, c = q % per * 8;
+    const typename I::raw* p = x + r * ld + c;
+    Vec16<E> v;
+    if (c + 8 <= n) {
+      typename I::raw t[8];
+      __builtin_memcpy(t, p, sizeof(t));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v.v[i] = E::put(I::get(t[i]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v.v[i] = c + i < n ? E::put(I::get(p[i])) : 0;
+    }
+    *(Vec16<E>*)(out + r * ldo + c) = v;
+  }
+}
+
+hipError_t launch_pad_rows(const void* x, int dtype_in, int64_t ld, int64_t rows, int64_t n, int dtype, void* out,
+                           int64_t ldo, hipStream_t stream) {
+  const int64_t blocks = (rows * (ldo / 8) + 255) / 256;
+  const unsigned grid = (unsigned)(blocks < 16384 ? blocks : 16384);
+  if (dtype_in == 0) {
+    if (dtype == 1)
+      pad_rows_kernel<BF16, F32><<<grid, 256, 0, stream>>>((const float*)x, ld, rows, n, (uint16_t*)out, ldo);
+    else
+      pad_rows_kernel<F16, F32><<<grid, 256, 0, stream>>>((const float*)x, ld, rows, n, (uint16_t*)out, ldo);
+  } else if (dtype == 1) {
+    pad_rows_kernel<BF16, BF16><<<grid, 256, 0, stream>>>((const uint16_t*)x, ld, rows, n, (uint16_t*)out, ldo);
+  } else {
+    pad_rows_kernel<F16, F16><<<grid, 256, 0, stream>>>((const uint16_t*)x, ld, rows, n, (uint16_t*)out, ldo);
+  }
+  return hipGetLastError();
 }
 
 }  // namespace bcjr

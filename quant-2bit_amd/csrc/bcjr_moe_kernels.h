@@ -80,6 +80,8 @@ struct GroupedParams {
   int64_t lda, ldb, a_rows, b_rows;
   int64_t M, N, K;
   int E;
+  // zeros follow the rows of a and b up to a multiple of 8 elements
+  bool zero_padded;
   int split;  // set by the launch
 };
 
@@ -109,6 +111,11 @@ hipError_t launch_grouped(const GroupedParams& P, int dtype, bool b_is_nk, hipSt
 // out (E, N, K) = a^T b over each group's rows, a (M, N), b (M, K) (rows of b
 // through P.rows); out in float32 or the operands' type.
 hipError_t launch_grouped_wgrad(const GroupedParams& P, int dtype, bool out_f32, hipStream_t stream);
+
+// Rows of n elements (float32 or of the 16-bit `dtype`) to rows of ldo (a
+// multiple of 8) of `dtype`, zeros behind them; out 16-byte aligned.
+hipError_t launch_pad_rows(const void* x, int dtype_in, int64_t ld, int64_t rows, int64_t n, int dtype, void* out,
+                           int64_t ldo, hipStream_t stream);
 
 enum { DISTILL_LOSS = 0, DISTILL_BACKWARD = 1, DISTILL_BOTH = 2 };
 constexpr int kDistillMaxVocab = 1 << 20;

@@ -160,6 +160,39 @@ RouteOut moe_route_autograd(const Tensor& logits, const OptTensor& valid, int64_
 
 // ----------------------------------------------------------- grouped products
 
+// Whether t's rows (of a 16-bit type) are 16-byte chunks: a row stride in eights and
+// an aligned start.  (By the offset in the storage, which tracing knows too; where
+// a storage itself is not aligned the slow kernel runs.)
+bool chunked(const Tensor& t) {
+  const int64_t d = t.dim();
+  return t.stride(d - 1) == 1 && t.stride(d - 2) % 8 == 0 && t.storage_offset() % 8 == 0;
+}
+// Row stride of rows with zeros behind them.
+int64_t chunk_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : (t.size(1) + 7) / 8 * 8; }
+
+// Rows (the last dimension) of t in `dtype` at a stride in eights with zeros
+// behind them: a view of t's sizes into a padded copy.
+Tensor padded(const Tensor& t, at::ScalarType dtype) {
+  const Tensor c = t.dim() == 2 ? strided_rows(t) : t.contiguous();
+  const int64_t n = t.size(-1), rows = n ? t.numel() / n : 0, ld = (n + 7) / 8 * 8;
+  auto sizes = t.sizes().vec();
+  sizes.back() = ld;
+  Tensor out = at::empty(sizes, t.options().dtype(dtype));
+  check(bcjr_pad_rows(c.data_ptr(), dtype_id(c, "x"), t.dim() == 2 ? row_stride(c) : n, rows, n, dtype_id(out, "x"),
+                      out.data_ptr(), ld, stream_of(t)),
+        "bcjr_pad_rows");
+  return out.narrow(-1, 0, n);
+}
+Tensor pad_rows_hip(const Tensor& t, const Tensor& like) {
+  const c10::OptionalDeviceGuard guard(at::device_of(t));
+  return padded(t, like.scalar_type());
+}
+Tensor pad_rows_meta(const Tensor& t, const Tensor& like) {
+  auto sizes = t.sizes().vec();
+  sizes.back() = (sizes.back() + 7) / 8 * 8;
+  return at::empty(sizes, t.options().dtype(like.scalar_type())).narrow(-1, 0, t.size(-1));
+}
+
 // Shapes of a product: x (T or M, K), w (E, N, K) or (E, K, N), offsets (E + 1), rows (M).
 struct Product {
   int64_t E, M, N, K;
@@ -176,24 +209,29 @@ Product product_args(const Tensor& x, const Tensor& w, const Tensor& offsets, co
   return p;
 }
 
+// zero_padded: x and w are chunked, with zeros behind rows that are not whole chunks.
 Tensor grouped_matmul_hip(const Tensor& x_in, const Tensor& w_in, const Tensor& offsets_in, const OptTensor& rows_in,
-                          bool w_is_nk) {
+                          bool w_is_nk, bool zero_padded) {
   const Product p = product_args(x_in, w_in, offsets_in, rows_in, w_is_nk);
   same_device(x_in, w_in, "w");
   same_device(x_in, offsets_in, "offsets");
   same_device(x_in, rows_in, "rows");
   const c10::OptionalDeviceGuard guard(at::device_of(x_in));
-  const Tensor x = strided_rows(x_in), w = w_in.contiguous(), offsets = as_int(offsets_in, "offsets");
+  const Tensor x = strided_rows(x_in), offsets = as_int(offsets_in, "offsets");
+  const bool rows_ok = w_in.stride(2) == 1 && w_in.stride(1) >= w_in.size(2) &&
+                       w_in.stride(0) == w_in.size(1) * w_in.stride(1);
+  const Tensor w = rows_ok ? w_in : w_in.contiguous();
   const OptTensor rows = as_int(rows_in, "rows");
   Tensor out = at::empty({p.M, p.N}, x.options());
-  check(bcjr_grouped_matmul(x.data_ptr(), dtype_id(x, "x"), row_stride(x), x.size(0), iptr(rows), w.data_ptr(),
-                            w_is_nk, offsets.data_ptr<int32_t>(), p.E, p.M, p.N, p.K, out.data_ptr(), stream_of(x)),
+  check(bcjr_grouped_matmul(x.data_ptr(), dtype_id(x, "x"), zero_padded ? chunk_stride(x) : row_stride(x), x.size(0),
+                            iptr(rows), w.data_ptr(), w.stride(1), w_is_nk, offsets.data_ptr<int32_t>(), p.E, p.M, p.N,
+                            p.K, zero_padded, out.data_ptr(), stream_of(x)),
         "bcjr_grouped_matmul");
   return out;
 }
 
 Tensor grouped_matmul_meta(const Tensor& x, const Tensor& w, const Tensor& offsets, const OptTensor& rows,
-                           bool w_is_nk) {
+                           bool w_is_nk, bool zero_padded) {
   const Product p = product_args(x, w, offsets, rows, w_is_nk);
   return at::empty({p.M, p.N}, x.options());
 }
@@ -207,7 +245,7 @@ void wgrad_args(const Tensor& gy, const Tensor& x, const Tensor& offsets, const 
 }
 
 Tensor grouped_wgrad_hip(const Tensor& gy_in, const Tensor& x_in, const Tensor& offsets_in, const OptTensor& rows_in,
-                         bool out_f32) {
+                         bool zero_padded, bool out_f32) {
   wgrad_args(gy_in, x_in, offsets_in, rows_in);
   same_device(x_in, gy_in, "gy");
   same_device(x_in, offsets_in, "offsets");
@@ -217,53 +255,78 @@ Tensor grouped_wgrad_hip(const Tensor& gy_in, const Tensor& x_in, const Tensor& 
   const OptTensor rows = as_int(rows_in, "rows");
   const int64_t E = offsets.size(0) - 1, M = gy.size(0), N = gy.size(1), K = x.size(1);
   Tensor out = at::empty({E, N, K}, out_f32 ? x.options().dtype(at::kFloat) : x.options());
-  check(bcjr_grouped_wgrad(gy.data_ptr(), dtype_id(x, "x"), row_stride(gy), x.data_ptr(), row_stride(x), x.size(0),
-                           iptr(rows), offsets.data_ptr<int32_t>(), E, M, N, K, out_f32, out.data_ptr(),
+  check(bcjr_grouped_wgrad(gy.data_ptr(), dtype_id(x, "x"), zero_padded ? chunk_stride(gy) : row_stride(gy), x.data_ptr(),
+                           zero_padded ? chunk_stride(x) : row_stride(x), x.size(0), iptr(rows),
+                           offsets.data_ptr<int32_t>(), E, M, N, K, zero_padded, out_f32, out.data_ptr(),
                            stream_of(x)),
         "bcjr_grouped_wgrad");
   return out;
 }
 
 Tensor grouped_wgrad_meta(const Tensor& gy, const Tensor& x, const Tensor& offsets, const OptTensor& rows,
-                          bool out_f32) {
+                          bool zero_padded, bool out_f32) {
   wgrad_args(gy, x, offsets, rows);
   return at::empty({offsets.size(0) - 1, gy.size(1), x.size(1)}, out_f32 ? x.options().dtype(at::kFloat) : x.options());
 }
 
-Tensor call_grouped(const Tensor& x, const Tensor& w, const Tensor& offsets, const OptTensor& rows, bool w_is_nk) {
+Tensor call_grouped(const Tensor& x, const Tensor& w, const Tensor& offsets, const OptTensor& rows, bool w_is_nk,
+                    bool zero_padded) {
   static auto op = c10::Dispatcher::singleton()
                        .findSchemaOrThrow("bcjr::grouped_product", "")
-                       .typed<Tensor(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, bool)>();
-  return op.call(x, w, offsets, rows, w_is_nk);
+                       .typed<Tensor(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, bool, bool)>();
+  return op.call(x, w, offsets, rows, w_is_nk, zero_padded);
+}
+
+Tensor call_wgrad(const Tensor& gy, const Tensor& x, const Tensor& offsets, const OptTensor& rows, bool zero_padded,
+                  bool out_f32) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("bcjr::grouped_wgrad", "")
+                       .typed<Tensor(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, bool, bool)>();
+  return op.call(gy, x, offsets, rows, zero_padded, out_f32);
+}
+
+Tensor call_pad(const Tensor& t, const Tensor& like) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("bcjr::pad_rows", "")
+                       .typed<Tensor(const Tensor&, const Tensor&)>();
+  return op.call(t, like);
 }
 
 Tensor call_combine(const Tensor& y, const OptTensor& weights, const Tensor& slots);
+
+// t in `like`'s type with rows of 16-byte chunks: t itself, a converted copy or a padded one.
+Tensor in_chunks(const Tensor& t, const Tensor& like) {
+  if (t.size(-1) % 8 == 0) {
+    const Tensor c = t.to(like.scalar_type());
+    if (chunked(c)) return c;
+  }
+  return call_pad(t, like);
+}
 
 struct GroupedFunction : torch::autograd::Function<GroupedFunction> {
   static Variable forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& offsets,
                           const OptTensor& rows, const OptTensor& slots) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    // the product's own copy of float32 weights, in the rows' type, serves the backward too
-    const Tensor wx = w.to(x.scalar_type());
-    ctx->save_for_backward({x, wx, offsets, rows ? *rows : Tensor(), slots ? *slots : Tensor()});
+    // copies of float32 weights and of rows that are not 16-byte chunks serve the backward too
+    const Tensor wx = in_chunks(w, x), xx = in_chunks(x, x);
+    ctx->save_for_backward({xx, wx, offsets, rows ? *rows : Tensor(), slots ? *slots : Tensor()});
     ctx->saved_data["w_f32"] = w.scalar_type() == at::kFloat;
-    return call_grouped(x, wx, offsets, rows, true);
+    return call_grouped(xx, wx, offsets, rows, true, x.size(1) % 8 != 0);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    static auto wgrad = c10::Dispatcher::singleton()
-                            .findSchemaOrThrow("bcjr::grouped_wgrad", "")
-                            .typed<Tensor(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, bool)>();
     const auto s = ctx->get_saved_variables();
     const Tensor &x = s[0], &w = s[1], &offsets = s[2];
     const OptTensor rows = s[3].defined() ? OptTensor(s[3]) : std::nullopt;
     Tensor gx, gw;
     if (g[0].defined()) {
+      const Tensor gy = in_chunks(g[0].dim() == 2 ? strided_rows(g[0]) : g[0], x);
+      const bool pad = x.size(1) % 8 != 0 || gy.size(1) % 8 != 0;
       if (ctx->needs_input_grad(0)) {
-        gx = call_grouped(g[0], w, offsets, std::nullopt, false);
+        gx = call_grouped(gy, w, offsets, std::nullopt, false, pad);
         // the places' gradients, rounded to the rows' type, summed in float32 over each row's places
         if (rows) gx = call_combine(gx, std::nullopt, s[4]);
       }
-      if (ctx->needs_input_grad(1)) gw = wgrad.call(g[0], x, offsets, rows, ctx->saved_data["w_f32"].toBool());
+      if (ctx->needs_input_grad(1)) gw = call_wgrad(gy, x, offsets, rows, pad, ctx->saved_data["w_f32"].toBool());
     }
     return {gx, gw, Tensor(), Tensor(), Tensor()};
   }
@@ -283,9 +346,18 @@ void grouped_args(const Tensor& x, const Tensor& w, const OptTensor& rows, const
 Tensor grouped_matmul(const Tensor& x, const Tensor& w, const Tensor& offsets, const OptTensor& rows,
                       const OptTensor& slots) {
   grouped_args(x, w, rows, slots);
-  if (wants_grad(x) || wants_grad(w)) return GroupedFunction::apply(x, w, offsets, rows, slots);
+  const bool half = x.scalar_type() != at::kFloat;
+  if (half && (wants_grad(x) || wants_grad(w))) return GroupedFunction::apply(x, w, offsets, rows, slots);
   at::AutoDispatchBelowADInplaceOrView guard;
-  return call_grouped(x, w.to(x.scalar_type()), offsets, rows, true);
+  const int64_t M = rows ? rows->numel() : x.size(0);
+  // Rows that are not 16-byte chunks: a padded copy of all weights pays once the
+  // experts have rows enough or the weights are small (or copied in any case);
+  // else the slow kernel reads the weights of the experts in use alone.  Padded /
+  // slow, microseconds, bfloat16: 64 experts of 1023 x 2047, 512 rows 175 / 145,
+  // 2,048 rows 183 / 253; 8 experts of 1001 x 1003, 8 rows 20 / 53.
+  if (half && (M >= 16 * w.size(0) || w.numel() < (1 << 25) || w.scalar_type() == at::kFloat))
+    return call_grouped(in_chunks(x, x), in_chunks(w, x), offsets, rows, true, x.size(1) % 8 != 0);
+  return call_grouped(x, w.to(x.scalar_type()), offsets, rows, true, false);
 }
 
 // -------------------------------------------------------------------- combine
@@ -515,8 +587,9 @@ TORCH_LIBRARY_FRAGMENT(bcjr, m) {
   m.def("moe_route(Tensor logits, Tensor? valid, int k, bool renormalize) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("moe_route_backward(Tensor logits, Tensor? valid, Tensor weights, Tensor experts, Tensor g_weights, "
         "bool renormalize) -> Tensor");
-  m.def("grouped_product(Tensor x, Tensor w, Tensor offsets, Tensor? rows, bool w_is_nk) -> Tensor");
-  m.def("grouped_wgrad(Tensor gy, Tensor x, Tensor offsets, Tensor? rows, bool out_f32) -> Tensor");
+  m.def("grouped_product(Tensor x, Tensor w, Tensor offsets, Tensor? rows, bool w_is_nk, bool zero_padded=False) -> Tensor");
+  m.def("grouped_wgrad(Tensor gy, Tensor x, Tensor offsets, Tensor? rows, bool zero_padded, bool out_f32) -> Tensor");
+  m.def("pad_rows(Tensor x, Tensor like) -> Tensor");
   m.def("combine(Tensor y, Tensor? weights, Tensor slots) -> Tensor");
   m.def("combine_backward(Tensor y, Tensor weights, Tensor rows, Tensor slots, Tensor g_out) -> (Tensor, Tensor)");
   m.def("topk_distill(Tensor logits, Tensor values, Tensor indices, Tensor? teacher_lse, float temperature, bool keep) "
@@ -536,6 +609,7 @@ TORCH_LIBRARY_IMPL(bcjr, CUDA, m) {
   m.impl("moe_route_backward", &moe_route_backward_hip);
   m.impl("grouped_product", &grouped_matmul_hip);
   m.impl("grouped_wgrad", &grouped_wgrad_hip);
+  m.impl("pad_rows", &pad_rows_hip);
   m.impl("combine", &moe_combine_hip);
   m.impl("combine_backward", &moe_combine_backward_hip);
   m.impl("topk_distill", &topk_distill_hip);
@@ -548,6 +622,7 @@ TORCH_LIBRARY_IMPL(bcjr, Meta, m) {
   m.impl("moe_route_backward", &moe_route_backward_meta);
   m.impl("grouped_product", &grouped_matmul_meta);
   m.impl("grouped_wgrad", &grouped_wgrad_meta);
+  m.impl("pad_rows", &pad_rows_meta);
   m.impl("combine", &moe_combine_meta);
   m.impl("combine_backward", &moe_combine_backward_meta);
   m.impl("topk_distill", &topk_distill_meta);

@@ -61,23 +61,42 @@ def test_route_workspace(lib):
     (2, 4, 8, 16, 1 << 21, -1, "K=2097152"),
 ])
 def test_grouped_refusals(lib, dtype, E, M, N, K, status, msg):
-    assert lib.bcjr_grouped_matmul(P, dtype, K, M, None, P, 1, P, E, M, N, K, P, None) == status
+    assert lib.bcjr_grouped_matmul(P, dtype, K, M, None, P, K, 1, P, E, M, N, K, 0, P, None) == status
     assert msg in _said(lib)
-    assert lib.bcjr_grouped_wgrad(P, dtype, N, P, K, M, None, P, E, M, N, K, 1, P, None) == status
+    assert lib.bcjr_grouped_wgrad(P, dtype, N, P, K, M, None, P, E, M, N, K, 0, 1, P, None) == status
     assert msg in _said(lib)
 
 
 def test_grouped_refuses_rows_and_strides(lib):
-    assert lib.bcjr_grouped_matmul(P, 1, 16, 7, None, P, 1, P, 4, 8, 16, 16, P, None) == -1
+    assert lib.bcjr_grouped_matmul(P, 1, 16, 7, None, P, 16, 1, P, 4, 8, 16, 16, 0, P, None) == -1
     assert "a has 7 rows for M=8" in _said(lib)
-    assert lib.bcjr_grouped_matmul(P, 1, 15, 8, None, P, 1, P, 4, 8, 16, 16, P, None) == -1
+    assert lib.bcjr_grouped_matmul(P, 1, 15, 8, None, P, 16, 1, P, 4, 8, 16, 16, 0, P, None) == -1
     assert "row stride 15" in _said(lib)
-    assert lib.bcjr_grouped_matmul(P, 1, 16, 8, None, None, 1, P, 4, 8, 16, 16, P, None) == -1
+    assert lib.bcjr_grouped_matmul(P, 1, 16, 8, None, P, 15, 1, P, 4, 8, 16, 16, 0, P, None) == -1
+    assert "row stride 15 of b" in _said(lib)
+    assert lib.bcjr_grouped_matmul(P, 1, 16, 8, None, None, 16, 1, P, 4, 8, 16, 16, 0, P, None) == -1
     assert "non-NULL" in _said(lib)
-    assert lib.bcjr_grouped_matmul(None, 1, 16, 0, None, None, 1, None, 4, 0, 16, 16, None, None) == 0
-    assert lib.bcjr_grouped_wgrad(P, 1, 16, P, 15, 8, None, P, 4, 8, 16, 16, 0, P, None) == -1
-    assert lib.bcjr_grouped_wgrad(P, 1, 15, P, 16, 8, None, P, 4, 8, 16, 16, 0, P, None) == -1
-    assert lib.bcjr_grouped_wgrad(P, 1, 16, P, 16, 7, None, P, 4, 8, 16, 16, 0, P, None) == -1
+    assert lib.bcjr_grouped_matmul(None, 1, 16, 0, None, None, 16, 1, None, 4, 0, 16, 16, 0, None, None) == 0
+    assert lib.bcjr_grouped_wgrad(P, 1, 16, P, 15, 8, None, P, 4, 8, 16, 16, 0, 0, P, None) == -1
+    assert lib.bcjr_grouped_wgrad(P, 1, 15, P, 16, 8, None, P, 4, 8, 16, 16, 0, 0, P, None) == -1
+    assert lib.bcjr_grouped_wgrad(P, 1, 16, P, 16, 7, None, P, 4, 8, 16, 16, 0, 0, P, None) == -1
+    # rows said to be padded that have no room for it
+    assert lib.bcjr_grouped_matmul(P, 1, 15, 8, None, P, 16, 1, P, 4, 8, 16, 15, 1, P, None) == -1
+    assert lib.bcjr_grouped_matmul(P, 1, 16, 8, None, P, 15, 1, P, 4, 8, 16, 15, 1, P, None) == -1
+    assert "in eights" in _said(lib)
+    assert lib.bcjr_grouped_wgrad(P, 1, 15, P, 16, 8, None, P, 4, 8, 15, 16, 1, 0, P, None) == -1
+
+
+def test_pad_rows_refusals(lib):
+    assert lib.bcjr_pad_rows(P, 0, 16, 4, 16, 0, P, 16, None) == -2
+    assert lib.bcjr_pad_rows(P, 2, 16, 4, 16, 1, P, 16, None) == -2
+    assert lib.bcjr_pad_rows(P, 0, 16, -1, 16, 1, P, 16, None) == -1
+    assert lib.bcjr_pad_rows(P, 0, 15, 4, 16, 1, P, 16, None) == -1
+    assert lib.bcjr_pad_rows(P, 0, 16, 4, 16, 1, P, 20, None) == -1
+    assert lib.bcjr_pad_rows(P, 0, 16, 4, 16, 1, P, 8, None) == -1
+    assert lib.bcjr_pad_rows(P, 0, 16, 4, 16, 1, ctypes.c_void_p(4104), 16, None) == -1
+    assert lib.bcjr_pad_rows(None, 0, 16, 4, 16, 1, P, 16, None) == -1
+    assert lib.bcjr_pad_rows(None, 0, 16, 0, 16, 1, None, 16, None) == 0
 
 
 def test_combine_refusals(lib):
