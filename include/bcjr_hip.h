@@ -360,8 +360,8 @@ int bcjr_moe_combine_backward(const void* y, int dtype, int64_t ldy, const float
  *   entries without it; p = softmax(logits / temperature);
  *   loss = sum q (log q - log p) + r (log r - log p_r), r = 1 - sum q (0 if
  *   under 1e-6 or without teacher_lse), p_r the student's mass outside the entries.
- * A row without entries has the loss 0 and the gradient 0.  stats (T, 4) keeps
- * what the backward needs, or NULL. */
+ * A row without entries has the loss 0 and the gradient 0.  stats (T, 8) keeps
+ * what the backward needs (16-byte aligned), or NULL. */
 int bcjr_topk_distill(const void* logits, int dtype, int64_t ld, const float* values,
                       const int32_t* indices, const float* teacher_lse, float temperature,
                       int64_t T, int64_t V, int64_t K, float* loss, float* stats,

@@ -12,9 +12,13 @@
 // them), not subtracted from 1, so a small one keeps its digits.
 //
 // One workgroup takes a row.  The loss reads it once, with a running maximum
-// and sum per thread; the gradient reads it again and writes it once, and
-// overwrites the K entries behind a barrier.  Exponents are base 2, sums
-// float32.  stats[row] = (log2-sum of z, c, c - r / p_r, n in log2 units).
+// and sum per thread; its last wave does the teacher's K entries meanwhile, whose
+// share of the loss needs the student's normaliser only as a factor.  The
+// gradient reads the row again and writes it once, and overwrites the K entries
+// behind a barrier; where loss and gradient are one call, a thread keeps its
+// first C vectors of the row in registers between the two.  Exponents are base 2
+// and of differences from the row's maximum m; sums are float32.
+// stats[row] = (m, log2 of the sum, c, c - r / p_r, n in log2 units, 3 unused).
 #include "bcjr_moe_device.h"
 #include "bcjr_moe_kernels.h"
 
@@ -22,8 +26,7 @@ namespace bcjr {
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kUnroll = 4;  // vectors in flight per thread
+constexpr int kUnroll = 4;  // vectors in flight per thread beside the kept ones
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // A teacher's mass outside its entries below this is what float32 sums leave of
 // 1 by rounding: none.
@@ -31,210 +34,258 @@ constexpr float kRest = 1e-6f;
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float lg2(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Running maximum, sum and sum outside the entries of one thread, z in log2 units.
+// Running maximum of logits, and sums of exponentials over it: all, and those
+// outside the entries.
 struct Run {
   float m = -INFINITY, l = 0.f, r = 0.f;
-  __device__ __forceinline__ void raise(float to) {
+  __device__ __forceinline__ void raise(float to, float s2) {
     if (to > m) {
-      const float f = ex2(m - to);  // 0 the first time
+      const float f = ex2((m - to) * s2);  // 0 the first time
       l *= f;
       r *= f;
       m = to;
     }
   }
-  __device__ __forceinline__ float ref() const { return m == -INFINITY ? 0.f : m; }
 };
 
-template <class E, int KIND, bool VEC>
-__global__ __launch_bounds__(kThreads) void distill_kernel(DistillParams P) {
-  constexpr int N = VEC ? Vec16<E>::N : 1;
+template <class E, int KIND, bool VEC, int NT, int C>
+__global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParams P) {
+  constexpr int N = VEC ? Vec16<E>::N : 1, NW = NT / 64;
   using raw = typename E::raw;
   extern __shared__ __align__(16) uint32_t marked[];  // one bit per element, from `lead` on
-  __shared__ float part[6][kWaves];
+  __shared__ float top[NW], part[2][NW], teacher[4];
   __shared__ int repeated;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
   const raw* x = (const raw*)P.logits + row * P.ld;
   raw* g = KIND == DISTILL_LOSS ? nullptr : (raw*)P.grad + row * P.V;
   const float* tv = P.values + row * P.K;
   const int32_t* ti = P.indices + row * P.K;
   const float s2 = P.inv_tau * kLog2e;  // logits to log2 units
-  const bool rest = P.teacher_lse != nullptr;
+  const bool rest = KIND != DISTILL_BACKWARD && P.teacher_lse != nullptr;
   // elements of the row's first 16-byte block that lie before the row
   const int lead = VEC ? (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(raw)) : 0;
   const int nvec = (P.V + lead + N - 1) / N;
-  const int words = (P.V + lead + 31) / 32;
   const int v0 = lead ? 1 : 0, v1 = (P.V + lead) / N;  // whole vectors
   const raw* xv = x - lead;
+  // threads 0 and 1 take the row's ends, inside vectors that it shares with its neighbours
+  const int edge = tid == 0 ? 0 : v1;
+  const bool has_edge = VEC && (tid == 0 ? v0 == 1 : tid == 1 && v1 < nvec && v1 >= v0);
+  auto entry = [&](int k) { return ti[k] >= 0 && ti[k] < P.V; };
 
-  const float gr = KIND == DISTILL_LOSS ? 0.f : P.g_rows[row];
-  for (int i = tid; i < words; i += kThreads) marked[i] = 0;
-  if (tid == 0) repeated = 0;
-  __syncthreads();
-  for (int k = tid; k < P.K; k += kThreads) {
-    const int i = ti[k];
-    if (i >= 0 && i < P.V) {
-      const uint32_t bit = 1u << ((i + lead) & 31);
-      if (atomicOr(&marked[(i + lead) >> 5], bit) & bit) repeated = 1;
-    }
+  if (KIND != DISTILL_LOSS || rest) {
+    const int words = (P.V + lead + 31) / 32;
+    for (int i = tid; i < words; i += NT) marked[i] = 0;
+    if (tid == 0) repeated = 0;
+    __syncthreads();
+    for (int k = tid; k < P.K; k += NT)
+      if (entry(k)) {
+        const int i = ti[k] + lead;
+        if (atomicOr(&marked[i >> 5], 1u << (i & 31)) >> (i & 31) & 1) repeated = 1;
+      }
+    __syncthreads();
   }
 
-  float lse2, c, outside, n2;
+  float m, L, c, outside, n2;  // m as it is subtracted
+  u32x4 keep[C > 0 ? C : 1];
+  auto vector_at = [&](int v) { return *(const u32x4*)(xv + (int64_t)v * N); };
   if constexpr (KIND == DISTILL_BACKWARD) {
-    const float4 s = P.stats[row];
-    lse2 = s.x, c = s.y, outside = s.z, n2 = s.w;
-    __syncthreads();
+    const float4 s = P.stats[2 * row];
+    m = s.x, L = s.y, c = s.z, outside = s.w;
+    n2 = P.stats[2 * row + 1].x;
   } else {
-    // the teacher's normaliser, log2 units
-    if (rest) {
-      n2 = P.teacher_lse[row] * kLog2e;
-      __syncthreads();
-    } else {
-      float m = -INFINITY, l = 0.f;
-      for (int k = tid; k < P.K; k += kThreads)
-        if (ti[k] >= 0 && ti[k] < P.V) m = fmaxf(m, tv[k] * s2);
-      m = group_max<kWaves>(m, part[0]);
-      const float ref = m == -INFINITY ? 0.f : m;
-      for (int k = tid; k < P.K; k += kThreads)
-        if (ti[k] >= 0 && ti[k] < P.V) l += ex2(tv[k] * s2 - ref);
-      l = group_sum<kWaves>(l, part[1]);
-      n2 = ref + lg2(l);  // -inf for a row without entries
-    }
-
     Run a;
-    auto add = [&](const float* z, uint32_t bits) {
-      const float ref = a.ref();
-      float s = 0.f;
+    // exponentials over a vector, and the same without the entries
+    auto add = [&](const float* z, int v) {
+      const float ref = finite_or_0(a.m);
+      float e[N], s = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) s += ex2(z[i] - ref);
+      for (int i = 0; i < N; ++i) s += e[i] = ex2((z[i] - ref) * s2);
       a.l += s;
       if (rest) {
+        const uint32_t bits = (marked[(v * N) >> 5] >> ((v * N) & 31)) & ((1u << N) - 1);
         if (bits) {
           s = 0.f;
 #pragma unroll
-          for (int i = 0; i < N; ++i) s += (bits >> i) & 1 ? 0.f : ex2(z[i] - ref);
+          for (int i = 0; i < N; ++i) s += (bits >> i) & 1 ? 0.f : e[i];
         }
         a.r += s;
       }
     };
-    auto bits_of = [&](int v) {
-      return rest ? (marked[(v * N) >> 5] >> ((v * N) & 31)) & ((1u << N) - 1) : 0u;
+    // Vector by vector in the same order whatever is kept, so that the loss alone
+    // and the loss beside its gradient have the same bits.
+    auto take = [&](const float* z, int v) {
+      float most = z[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) most = fmaxf(most, z[i]);
+      a.raise(most, s2);
+      add(z, v);
     };
-    for (int v = v0 + tid; v < v1; v += kThreads * kUnroll) {
-      float z[kUnroll][N];
-      int nv = 0;
-      float m = -INFINITY;
+    int v = v0 + tid;
+    if constexpr (VEC) {
+      if constexpr (C > 0) {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if (v + u * kThreads >= v1) break;
-        nv = u + 1;
-        if constexpr (VEC) {
-          const Vec16<E> t = *(const Vec16<E>*)(xv + (int64_t)(v + u * kThreads) * N);
+        for (int u = 0; u < C; ++u)
+          if (v + u * NT < v1) keep[u] = vector_at(v + u * NT);
 #pragma unroll
-          for (int i = 0; i < N; ++i) z[u][i] = E::get(t.v[i]);
-        } else {
-          z[u][0] = E::get(xv[v + u * kThreads]);
+        for (int u = 0; u < C; ++u)
+          if (v + u * NT < v1) {
+            float z[N];
+            unpack16<E>(keep[u], z);
+            take(z, v + u * NT);
+          }
+        v += C * NT;
+      }
+      for (; v + (kUnroll - 1) * NT < v1; v += kUnroll * NT) {
+        u32x4 t[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) t[u] = vector_at(v + u * NT);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          float z[N];
+          unpack16<E>(t[u], z);
+          take(z, v + u * NT);
         }
       }
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if (u >= nv) break;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          z[u][i] *= s2;
-          m = fmaxf(m, z[u][i]);
-        }
+      for (; v < v1; v += NT) {
+        float z[N];
+        unpack16<E>(vector_at(v), z);
+        take(z, v);
       }
-      a.raise(m);
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if (u >= nv) break;
-        add(z[u], bits_of(v + u * kThreads));
+    } else {
+      for (; v < v1; v += NT) {
+        const float z = E::get(xv[v]);
+        take(&z, v);
       }
     }
-    // the row's ends, inside vectors that it shares with its neighbours
-    if (VEC && tid < 2) {
-      const int v = tid == 0 ? 0 : v1;
-      if ((tid == 0 ? v0 == 1 : v1 < nvec && v1 >= v0) ) {
-        float z[N], m = -INFINITY;
+    if (has_edge) {
+      float z[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int e = v * N + i - lead;
-          z[i] = e >= 0 && e < P.V ? E::get(x[e]) * s2 : -INFINITY;
-          m = fmaxf(m, z[i]);
-        }
-        a.raise(m);
-        add(z, bits_of(v));
+      for (int i = 0; i < N; ++i) {
+        const int e = edge * N + i - lead;
+        z[i] = e >= 0 && e < P.V ? E::get(x[e]) : -INFINITY;
       }
+      take(z, edge);
     }
-    const float m = group_max<kWaves>(a.m, part[2]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    const float f = ex2(a.ref() - ref);
-    const float total = group_sum<kWaves>(a.m == -INFINITY ? a.l : a.l * f, part[3]);
-    lse2 = ref + lg2(total);
 
-    // the entries
-    float term = 0.f, mass = 0.f;
-    for (int k = tid; k < P.K; k += kThreads) {
-      const int i = ti[k];
-      if (i < 0 || i >= P.V) continue;
-      const float lq = tv[k] * s2 - n2, q = ex2(lq);
-      mass += q;
-      if (q != 0.f) term += q * (lq - (E::get(x[i]) * s2 - lse2)) * kLn2;
+    // The entries, by one wave: n2, sum q, the largest student logit x_k among
+    // them and sum q (log q - (x - x_k)).
+    if (wave == NW - 1) {
+      float most = -INFINITY;
+      if (rest) {
+        n2 = P.teacher_lse[row] * kLog2e;
+      } else {
+        float l = 0.f;
+        for (int k = lane; k < P.K; k += 64)
+          if (entry(k)) most = fmaxf(most, tv[k]);
+        const float ref = finite_or_0(wave_max(most));
+        for (int k = lane; k < P.K; k += 64)
+          if (entry(k)) l += ex2((tv[k] - ref) * s2);
+        n2 = ref * s2 + lg2(wave_sum(l));  // -inf for a row without entries
+      }
+      most = -INFINITY;
+      for (int k = lane; k < P.K; k += 64)
+        if (entry(k)) most = fmaxf(most, E::get(x[ti[k]]));
+      const float xk = finite_or_0(wave_max(most));
+      float mass = 0.f, term = 0.f;
+      for (int k = lane; k < P.K; k += 64)
+        if (entry(k)) {
+          const float lq = tv[k] * s2 - n2, q = ex2(lq);
+          mass += q;
+          if (q != 0.f) term += q * (lq - (E::get(x[ti[k]]) - xk) * s2);
+        }
+      mass = wave_sum(mass);
+      term = wave_sum(term);
+      if (lane == 0) teacher[0] = n2, teacher[1] = mass, teacher[2] = term, teacher[3] = xk;
     }
-    term = group_sum<kWaves>(term, part[4]);
-    mass = group_sum<kWaves>(mass, part[5]);
+    const float wm = wave_max(a.m);
+    if (lane == 0) top[wave] = wm;
+    __syncthreads();
+    m = top[0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) m = fmaxf(m, top[i]);
+    m = finite_or_0(m);
+    const float f = a.m == -INFINITY ? 1.f : ex2((a.m - m) * s2);
+    const float wl = wave_sum(a.l * f), wr = rest ? wave_sum(a.r * f) : 0.f;
+    if (lane == 0) part[0][wave] = wl, part[1][wave] = wr;
+    __syncthreads();
+    float total = 0.f, others = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      total += part[0][i];
+      if (rest) others += part[1][i];
+    }
+    L = lg2(total);
+    n2 = teacher[0];
+    const float mass = teacher[1];
+    float loss = mass == 0.f ? 0.f : (teacher[2] + mass * ((m - teacher[3]) * s2 + L)) * kLn2;
     outside = c = rest ? mass : (n2 == -INFINITY ? 0.f : 1.f);
     if (rest) {
-      __syncthreads();
-      const float pr = group_sum<kWaves>(a.m == -INFINITY ? a.r : a.r * f, part[0]) / total;
+      const float pr = others / total;
       float r = 1.f - mass;
       r = r > kRest ? r : 0.f;
       c = mass + r;
       outside = c;
       if (r > 0.f) {
-        term += r * (lg2(r) - lg2(pr)) * kLn2;
+        loss += r * (lg2(r) - lg2(pr)) * kLn2;
         if (pr > 0.f) outside = c - r / pr;
       }
     }
-    if (c == 0.f) term = 0.f;  // no entries
+    if (c == 0.f) loss = 0.f;  // no entries
     if (tid == 0) {
-      P.loss[row] = term;
-      if (P.stats) P.stats[row] = make_float4(lse2, c, outside, n2);
+      P.loss[row] = loss;
+      if (P.stats) {
+        P.stats[2 * row] = make_float4(m, L, c, outside);
+        P.stats[2 * row + 1] = make_float4(n2, 0.f, 0.f, 0.f);
+      }
     }
   }
 
   if constexpr (KIND != DISTILL_LOSS) {
-    const float scale = gr * P.inv_tau;
+    const float scale = P.g_rows[row] * P.inv_tau;
     // rows that count nothing: zeros, whatever their logits are
     const bool none = scale == 0.f || c == 0.f;
     const float go = scale * outside;
-    auto out = [&](float z) { return none ? 0.f : ex2(fmaf(z, s2, -lse2)) * go; };
-    for (int v = v0 + tid; v < v1; v += kThreads) {
-      if constexpr (VEC) {
-        Vec16<E> t = {};
-        if (!none) t = *(const Vec16<E>*)(xv + (int64_t)v * N);
+    auto p_of = [&](float z) { return ex2(fmaf(z - m, s2, -L)); };
+    auto out = [&](float z) { return none ? 0.f : p_of(z) * go; };
+    auto write = [&](int v, u32x4 t) {
+      float z[N];
+      unpack16<E>(t, z);
 #pragma unroll
-        for (int i = 0; i < N; ++i) t.v[i] = E::put(out(E::get(t.v[i])));
-        *(Vec16<E>*)(g - lead + (int64_t)v * N) = t;
-      } else {
-        g[v] = E::put(out(E::get(x[v])));
+      for (int i = 0; i < N; ++i) z[i] = out(z[i]);
+      *(u32x4*)(g - lead + (int64_t)v * N) = pack16<E>(z);
+    };
+    int v = v0 + tid;
+    if constexpr (VEC) {
+      if constexpr (C > 0) {
+        // (else the compiler keeps the 16-bit types' elements apart, in twice the registers)
+#pragma unroll
+        for (int u = 0; u < C; ++u) asm volatile("" : "+v"(keep[u]));
+#pragma unroll
+        for (int u = 0; u < C; ++u)
+          if (v + u * NT < v1) write(v + u * NT, keep[u]);
+        v += C * NT;
       }
+      for (; v < v1; v += NT) {
+        u32x4 t = {0, 0, 0, 0};
+        if (!none) t = vector_at(v);
+        write(v, t);
+      }
+    } else {
+      for (; v < v1; v += NT) g[v] = E::put(out(E::get(x[v])));
     }
-    if (VEC && tid < 2) {
-      const int v = tid == 0 ? 0 : v1;
-      if ((tid == 0 ? v0 == 1 : v1 < nvec && v1 >= v0))
-        for (int i = 0; i < N; ++i) {
-          const int e = v * N + i - lead;
-          if (e >= 0 && e < P.V) g[e] = E::put(out(E::get(x[e])));
-        }
-    }
+    if (has_edge)
+      for (int i = 0; i < N; ++i) {
+        const int e = edge * N + i - lead;
+        if (e >= 0 && e < P.V) g[e] = E::put(out(E::get(x[e])));
+      }
     if (none) return;
     __syncthreads();
-    for (int k = tid; k < P.K; k += kThreads) {
+    for (int k = tid; k < P.K; k += NT) {
+      if (!entry(k)) continue;
       const int i = ti[k];
-      if (i < 0 || i >= P.V) continue;
       float q = 0.f;
       if (!repeated) {
         q = ex2(tv[k] * s2 - n2);
@@ -242,16 +293,37 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(DistillParams P) {
         for (int o = 0; o < P.K; ++o)
           if (ti[o] == i) q += ex2(tv[o] * s2 - n2);
       }
-      g[i] = E::put(scale * (ex2(fmaf(E::get(x[i]), s2, -lse2)) * c - q));
+      g[i] = E::put(scale * (p_of(E::get(x[i])) * c - q));
     }
   }
 }
 
-template <class E, bool VEC>
-const void* distill_ptr(int kind) {
-  return kind == DISTILL_LOSS       ? (const void*)distill_kernel<E, DISTILL_LOSS, VEC>
-         : kind == DISTILL_BACKWARD ? (const void*)distill_kernel<E, DISTILL_BACKWARD, VEC>
-                                    : (const void*)distill_kernel<E, DISTILL_BOTH, VEC>;
+// Threads of a row's workgroup, by its number of 16-byte vectors, for the loss and
+// for the loss with its gradient (one rule, so that their bits agree).  Small
+// workgroups let rows overlap their beginnings and ends; large ones keep more of a
+// long row on the chip between its two uses.  Loss with gradient, microseconds,
+// 256 threads keeping 12 vectors / 512 keeping 16 / 1,024 keeping 16:
+//   8,192 rows of  8,000 float32  (2,000 vectors)   105 /  143 /  234
+//   1,024 rows of 32,000 bfloat16 (4,000)            30 /   33 /   44
+//   4,096 rows of 50,257 bfloat16 (6,282)           214 /  197 /  237
+//   8,192 rows of 131,072 bfloat16 (16,384)       1,211 /  981 / 1,022
+//   4,096 rows of 131,072 float32 (32,768)        1,217 / 1,114 /  913
+// (keeping none: 140, 34, 218, 1,055 and 1,166 at the best width of each).
+int row_threads(int64_t nvec) { return nvec < 3000 ? 256 : nvec <= 16384 ? 512 : 1024; }
+
+template <class E>
+const void* distill_ptr(int kind, bool vec, int nt) {
+  if (kind == DISTILL_BACKWARD)
+    return vec ? (const void*)distill_kernel<E, DISTILL_BACKWARD, true, 1024, 0>
+               : (const void*)distill_kernel<E, DISTILL_BACKWARD, false, 1024, 0>;
+  if (kind == DISTILL_LOSS)
+    return nt == 256   ? (const void*)distill_kernel<E, DISTILL_LOSS, true, 256, 0>
+           : nt == 512 ? (const void*)distill_kernel<E, DISTILL_LOSS, true, 512, 0>
+                       : (const void*)distill_kernel<E, DISTILL_LOSS, true, 1024, 0>;
+  if (!vec) return (const void*)distill_kernel<E, DISTILL_BOTH, false, 1024, 0>;
+  return nt == 256   ? (const void*)distill_kernel<E, DISTILL_BOTH, true, 256, 12>
+         : nt == 512 ? (const void*)distill_kernel<E, DISTILL_BOTH, true, 512, 16>
+                     : (const void*)distill_kernel<E, DISTILL_BOTH, true, 1024, 16>;
 }
 
 }  // namespace
@@ -262,15 +334,16 @@ hipError_t launch_distill(const DistillParams& P, int dtype, int kind, hipStream
   const bool vec = kind == DISTILL_LOSS ||
                    (((reinterpret_cast<uintptr_t>(P.logits) ^ reinterpret_cast<uintptr_t>(P.grad)) & 15) == 0 &&
                     (P.T == 1 || (P.ld - P.V) * (int64_t)es % 16 == 0));
-  const void* fn = dtype == 0   ? (vec ? distill_ptr<F32, true>(kind) : distill_ptr<F32, false>(kind))
-                   : dtype == 1 ? (vec ? distill_ptr<BF16, true>(kind) : distill_ptr<BF16, false>(kind))
-                                : (vec ? distill_ptr<F16, true>(kind) : distill_ptr<F16, false>(kind));
-  const size_t lds = ((size_t)P.V + 8 + 31) / 32 * 4 + 16;
+  const int nt = kind == DISTILL_BACKWARD || !vec ? 1024 : row_threads((int64_t)P.V * (int64_t)es / 16);
+  const void* fn = dtype == 0   ? distill_ptr<F32>(kind, vec, nt)
+                   : dtype == 1 ? distill_ptr<BF16>(kind, vec, nt)
+                                : distill_ptr<F16>(kind, vec, nt);
+  const size_t lds = kind == DISTILL_LOSS && !P.teacher_lse ? 0 : ((size_t)P.V + 8 + 31) / 32 * 4 + 16;
   hipError_t e = hipSuccess;
   if (lds > 60000) e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (e != hipSuccess) return e;
   void* args[] = {(void*)&P};
-  return hipLaunchKernel(fn, dim3((unsigned)P.T), dim3(kThreads), args, lds, stream);
+  return hipLaunchKernel(fn, dim3((unsigned)P.T), dim3(nt), args, lds, stream);
 }
 
 }  // namespace bcjr

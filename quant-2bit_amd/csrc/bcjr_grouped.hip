@@ -215,7 +215,6 @@ __global__ __launch_bounds__(256) void wgrad_any_kernel(GroupedParams P) {
 // are permuted by its number so that the 16 lanes of a read's pass meet
 // distinct banks.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBK = 64;
 constexpr int kFastThreads = 512;

@@ -36,6 +36,34 @@ struct alignas(16) Vec16 {
   typename E::raw v[N];
 };
 
+// The same 16 bytes as four registers, and their elements.  (Arrays of 16-bit
+// elements that live long are kept one to a register.)
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <class E>
+__device__ __forceinline__ void unpack16(u32x4 v, float* z) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(typename E::raw) == 4) {
+      z[i] = __uint_as_float(v[i]);
+    } else {
+      z[2 * i] = E::get((typename E::raw)(v[i] & 0xffffu));
+      z[2 * i + 1] = E::get((typename E::raw)(v[i] >> 16));
+    }
+  }
+}
+template <class E>
+__device__ __forceinline__ u32x4 pack16(const float* z) {
+  u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(typename E::raw) == 4)
+      v[i] = __float_as_uint(z[i]);
+    else
+      v[i] = (uint32_t)E::put(z[2 * i]) | (uint32_t)E::put(z[2 * i + 1]) << 16;
+  }
+  return v;
+}
+
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));

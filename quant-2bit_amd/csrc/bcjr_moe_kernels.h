@@ -92,7 +92,7 @@ struct DistillParams {
   const float* teacher_lse; // (T) or null
   const float* g_rows;      // (T): gradient of each row's loss
   float* loss;              // (T)
-  float4* stats;            // (T): see bcjr_distill.hip
+  float4* stats;            // (T, 2): see bcjr_distill.hip
   void* grad;               // (T, V)
   int64_t T, ld;
   int V, K;

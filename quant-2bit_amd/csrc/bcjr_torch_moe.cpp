@@ -484,13 +484,13 @@ Distill distill_inputs(const Tensor& logits, const Tensor& values, const Tensor&
 
 const float* lse_ptr(const Distill& d) { return d.lse.defined() ? d.lse.data_ptr<float>() : nullptr; }
 
-// loss (T,) and, with keep, stats (T, 4) for the backward (else (0, 4)).
+// loss (T,) and, with keep, stats (T, 8) for the backward (else (0, 8)).
 std::tuple<Tensor, Tensor> topk_distill_hip(const Tensor& logits, const Tensor& values, const Tensor& indices,
                                             const OptTensor& lse, double temperature, bool keep) {
   const c10::OptionalDeviceGuard guard(at::device_of(logits));
   const Distill d = distill_inputs(logits, values, indices, lse);
   const auto f32 = logits.options().dtype(at::kFloat);
-  Tensor loss = at::empty({d.T}, f32), stats = at::empty({keep ? d.T : 0, 4}, f32);
+  Tensor loss = at::empty({d.T}, f32), stats = at::empty({keep ? d.T : 0, 8}, f32);
   check(bcjr_topk_distill(d.logits.data_ptr(), d.dtype, row_stride(d.logits), d.values.data_ptr<float>(),
                           d.indices.data_ptr<int32_t>(), lse_ptr(d), (float)temperature, d.T, d.V, d.K,
                           loss.data_ptr<float>(), keep ? stats.data_ptr<float>() : nullptr, stream_of(logits)),
@@ -502,7 +502,7 @@ std::tuple<Tensor, Tensor> topk_distill_meta(const Tensor& logits, const Tensor&
                                              const OptTensor& lse, double temperature, bool keep) {
   distill_args(logits, values, indices, lse);
   const auto f32 = logits.options().dtype(at::kFloat);
-  return {at::empty({logits.size(0)}, f32), at::empty({keep ? logits.size(0) : 0, 4}, f32)};
+  return {at::empty({logits.size(0)}, f32), at::empty({keep ? logits.size(0) : 0, 8}, f32)};
 }
 
 Tensor topk_distill_backward_hip(const Tensor& logits, const Tensor& values, const Tensor& indices,
