@@ -46,7 +46,7 @@ int check_routing(int dtype, int64_t ld, int64_t T, int64_t E, int k) {
 }
 
 size_t route_ws(int64_t T, int64_t E) {
-  return T <= bcjr::kRouteOneBlock ? 0 : (size_t)bcjr::route_blocks(T, E) * (size_t)E * sizeof(int32_t);
+  return T <= bcjr::kRouteOneBlock ? 0 : (size_t)(bcjr::route_blocks(T) + 1) * (size_t)E * sizeof(int32_t);
 }
 
 constexpr int64_t kMaxDim = 1 << 20;
@@ -62,14 +62,19 @@ int check_grouped(int dtype, int64_t E, int64_t M, int64_t N, int64_t K) {
   if (M < 0 || M > INT32_MAX) return fail(BCJR_EINVAL, "M=%lld rows outside [0, 2^31)", (ll)M);
   if (N < 1 || N > kMaxDim || K < 1 || K > kMaxDim)
     return fail(BCJR_EINVAL, "N=%lld, K=%lld must be in [1, %lld]", (ll)N, (ll)K, (ll)kMaxDim);
+  // a launch has fewer than 2^32 threads, 512 a tile of 256 x 256
+  const int64_t most = 1 << 23, n = N / 256 + 1, k = K / 256 + 1;
+  if ((M / 256 + E + 1) * (n > k ? n : k) >= most || E * n * k >= most || M >= 1 << 30)
+    return fail(BCJR_EUNSUPPORTED, "M=%lld, N=%lld, K=%lld, E=%lld: more tiles than a launch holds", (ll)M, (ll)N, (ll)K,
+                (ll)E);
   return BCJR_OK;
 }
 
 int check_combine(int dtype, int64_t ldy, int64_t T, int k, int64_t M, int64_t N) {
   if (int rc = check_dtype(dtype)) return rc;
   if (k < 1) return fail(BCJR_EINVAL, "k=%d must be >= 1", k);
-  if (T < 0 || M < 0 || M > INT32_MAX || T > INT32_MAX)
-    return fail(BCJR_EINVAL, "T=%lld tokens, M=%lld rows outside [0, 2^31)", (ll)T, (ll)M);
+  if (T < 0 || M < 0 || M > INT32_MAX) return fail(BCJR_EINVAL, "T=%lld tokens, M=%lld rows outside [0, 2^31)", (ll)T, (ll)M);
+  if (T >= 1 << 24) return fail(BCJR_EUNSUPPORTED, "T=%lld tokens: combine is built for fewer than 2^24", (ll)T);
   if (N < 1 || N > kMaxDim) return fail(BCJR_EINVAL, "N=%lld must be in [1, %lld]", (ll)N, (ll)kMaxDim);
   if (M > 1 && ldy < N) return fail(BCJR_EINVAL, "row stride %lld is below N=%lld", (ll)ldy, (ll)N);
   return BCJR_OK;
@@ -79,7 +84,8 @@ int check_distill(int dtype, int64_t ld, float temperature, int64_t T, int64_t V
   if (int rc = check_dtype(dtype)) return rc;
   if (!(temperature > 0.f) || !std::isfinite(temperature) || !std::isfinite(1.f / temperature))
     return fail(BCJR_EINVAL, "temperature %g must be finite and > 0", (double)temperature);
-  if (T < 0 || T > INT32_MAX) return fail(BCJR_EINVAL, "T=%lld rows outside [0, 2^31)", (ll)T);
+  if (T < 0) return fail(BCJR_EINVAL, "T=%lld rows must be >= 0", (ll)T);
+  if (T >= 1 << 22) return fail(BCJR_EUNSUPPORTED, "T=%lld rows: the loss is built for fewer than 2^22", (ll)T);
   if (V < 1 || V > bcjr::kDistillMaxVocab)
     return fail(V < 1 ? BCJR_EINVAL : BCJR_EUNSUPPORTED, "V=%lld outside [1, %d]", (ll)V, bcjr::kDistillMaxVocab);
   if (K < 0 || K > V) return fail(BCJR_EINVAL, "K=%lld teacher entries outside [0, V=%lld]", (ll)K, (ll)V);

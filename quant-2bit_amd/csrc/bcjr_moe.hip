@@ -15,7 +15,9 @@
 // of the counts before it.  Equal calls give equal results.
 //
 // Up to kRouteOneBlock tokens one launch does all; more take two, one for the
-// picks and the counts of every block, one for the places.
+// picks and the counts of every block, one for the places, whose blocks sum the
+// counts before their own; above 256 blocks that would read too much, and a
+// launch between the two sums them once.
 #include <algorithm>
 
 #include "bcjr_moe_device.h"
@@ -173,7 +175,33 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteParams P) {
   }
 }
 
-// The places of one block's pairs; every block sums the counts it needs.
+// counts[block][e] becomes the sum of the blocks before it; the totals follow
+// behind the last block.  A workgroup takes 64 experts, its waves parts of the
+// blocks.
+__global__ __launch_bounds__(kThreads) void route_scan_kernel(int32_t* counts, int nb, int E) {
+  constexpr int kParts = kThreads / 64;
+  __shared__ int sums[kParts][64];
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
+  const int per = (nb + kParts - 1) / kParts, b0 = min(part * per, nb), b1 = min(b0 + per, nb);
+  int sum = 0;
+  if (e < E)
+    for (int b = b0; b < b1; ++b) sum += counts[(size_t)b * E + e];
+  sums[part][lane] = sum;
+  __syncthreads();
+  int at = 0;
+  for (int p = 0; p < part; ++p) at += sums[p][lane];
+  if (e >= E) return;
+  for (int b = b0; b < b1; ++b) {
+    const int c = counts[(size_t)b * E + e];
+    counts[(size_t)b * E + e] = at;
+    at += c;
+  }
+  if (part == kParts - 1) counts[(size_t)nb * E + e] = at;
+}
+
+// The places of one block's pairs.  Unless SCANNED, every block sums the counts
+// it needs.
+template <bool SCANNED>
 __global__ __launch_bounds__(kThreads) void route_place_kernel(RouteParams P) {
   extern __shared__ __align__(16) char lds[];
   unsigned long long* mask = (unsigned long long*)lds;
@@ -185,19 +213,27 @@ __global__ __launch_bounds__(kThreads) void route_place_kernel(RouteParams P) {
   for (int i = tid; i < P.E * P.words; i += kThreads) mask[i] = 0;
   for (int e = tid; e < P.E; e += kThreads) start[e] = before[e] = 0;
   __syncthreads();
-  // a wave sums 64 experts' counts over every nparts-th block
-  const int nb = gridDim.x, groups = (P.E + 63) / 64, nparts = max(1, kThreads / 64 / groups);
-  for (int wg = tid >> 6; wg < groups * nparts; wg += kThreads / 64) {
-    const int e = wg % groups * 64 + (tid & 63), part = wg / groups;
-    if (e < P.E) {
-      int all = 0, mine = 0;
-      for (int b = part; b < nb; b += nparts) {
-        const int c = P.counts[(size_t)b * P.E + e];
-        all += c;
-        if (b < (int)blockIdx.x) mine += c;
+  const int nb = gridDim.x;
+  if (SCANNED) {
+    for (int e = tid; e < P.E; e += kThreads) {
+      before[e] = P.counts[(size_t)blockIdx.x * P.E + e];
+      start[e] = P.counts[(size_t)nb * P.E + e];
+    }
+  } else {
+    // a wave sums 64 experts' counts over every nparts-th block
+    const int groups = (P.E + 63) / 64, nparts = max(1, kThreads / 64 / groups);
+    for (int wg = tid >> 6; wg < groups * nparts; wg += kThreads / 64) {
+      const int e = wg % groups * 64 + (tid & 63), part = wg / groups;
+      if (e < P.E) {
+        int all = 0, mine = 0;
+        for (int b = part; b < nb; b += nparts) {
+          const int c = P.counts[(size_t)b * P.E + e];
+          all += c;
+          if (b < (int)blockIdx.x) mine += c;
+        }
+        atomicAdd(&start[e], all);  // whole numbers: the order does not matter
+        atomicAdd(&before[e], mine);
       }
-      atomicAdd(&start[e], all);  // whole numbers: the order does not matter
-      atomicAdd(&before[e], mine);
     }
   }
   const int64_t p0 = t0 * P.k;
@@ -422,7 +458,7 @@ bool aligned(const void* p, int64_t ld, int dtype) {
 hipError_t launch_route(RouteParams P, int dtype, hipStream_t stream) {
   const int v = route_variant(P.E, P.k);
   const bool one = P.T <= kRouteOneBlock;
-  const int words = one ? (int)std::max<int64_t>(1, (P.T + 63) / 64) : route_words(P.T, P.E);
+  const int words = one ? (int)std::max<int64_t>(1, (P.T + 63) / 64) : route_words(P.T);
   P.words = words;
   const unsigned nb = (unsigned)std::max<int64_t>(1, (P.T + words * 64 - 1) / (words * 64));
   const size_t lds = (size_t)P.E * words * 8 + (2 * (size_t)P.E + 1) * 4;
@@ -433,10 +469,18 @@ hipError_t launch_route(RouteParams P, int dtype, hipStream_t stream) {
   void* args[] = {&P};
   e = hipLaunchKernel(fn, dim3(nb), dim3(kThreads), args, lds, stream);
   if (e != hipSuccess || one) return e;
-  if (lds > 65536)
-    e = hipFuncSetAttribute((const void*)route_place_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  const bool scan = nb > 256;
+  if (scan) {
+    int n = (int)nb;
+    void* sargs[] = {&P.counts, &n, &P.E};
+    e = hipLaunchKernel((const void*)route_scan_kernel, dim3((unsigned)((P.E + 63) / 64)), dim3(kThreads), sargs, 0,
+                        stream);
+    if (e != hipSuccess) return e;
+  }
+  fn = scan ? (const void*)route_place_kernel<true> : (const void*)route_place_kernel<false>;
+  if (lds > 65536) e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (e != hipSuccess) return e;
-  return hipLaunchKernel((const void*)route_place_kernel, dim3(nb), dim3(kThreads), args, lds, stream);
+  return hipLaunchKernel(fn, dim3(nb), dim3(kThreads), args, lds, stream);
 }
 
 hipError_t launch_route_backward(const RouteBwdParams& P, int dtype, hipStream_t stream) {

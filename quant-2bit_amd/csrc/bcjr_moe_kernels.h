@@ -16,13 +16,12 @@ constexpr int kRouteMaxPicks = 64;
 
 // 64-token words of a routing block: one (64 tokens) up to 16,384 tokens, so
 // that the chip is full, then as many as keep 256 blocks, at most 16.
-inline int route_words(int64_t T, int64_t E) {
-  (void)E;
+inline int route_words(int64_t T) {
   const int64_t w = (T + 64 * 256 - 1) / (64 * 256);
   return (int)(w < 1 ? 1 : w > 16 ? 16 : w);
 }
-inline int64_t route_blocks(int64_t T, int64_t E) {
-  const int64_t per = 64 * (int64_t)route_words(T, E);
+inline int64_t route_blocks(int64_t T) {
+  const int64_t per = 64 * (int64_t)route_words(T);
   return (T + per - 1) / per;
 }
 
@@ -34,7 +33,7 @@ struct RouteParams {
   int32_t* offsets;      // (E + 1)
   int32_t* rows;         // (T * k)
   int32_t* slots;        // (T, k)
-  int32_t* counts;       // (blocks, E): workspace of the two-launch form
+  int32_t* counts;       // (blocks + 1, E): workspace of more than one block
   int64_t T, ld;
   int E, k, renormalize, words;
 };

@@ -562,3 +562,52 @@ def test_layer_trains_quantized_experts(bcjr_mod):
     out.float().square().sum().backward()
     for t in lat + [router]:
         assert t.grad is not None and torch.isfinite(t.grad).all() and (t.grad != 0).any()
+
+
+def test_layer_compiles_whole(bcjr_mod):
+    """torch.compile traces a layer's forward and backward without a graph break."""
+    g = gen(43)
+    T, E, k, H, I = 40, 6, 2, 64, 48
+    x = torch.randn(T, H, device=DEV, generator=g).bfloat16().requires_grad_()
+    router = torch.randn(E, H, device=DEV, generator=g) / 8
+    wgu = (torch.randn(E, 2 * I, H, device=DEV, generator=g) / 8).requires_grad_()
+    wd = (torch.randn(E, H, I, device=DEV, generator=g) / 8).requires_grad_()
+    idx = torch.randint(0, H, (T, 5), device=DEV, generator=g)
+    val = torch.randn(T, 5, device=DEV, generator=g)
+
+    def step(x, wgu, wd):
+        out = _layer(bcjr_mod, x, router, wgu, wd, k)
+        return bcjr_mod.topk_distill_loss(out, val, idx, temperature=2.0).mean()
+
+    want = step(x, wgu, wd)
+    gw = torch.autograd.grad(want, (x, wgu, wd))
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(x, wgu, wd)
+    gg = torch.autograd.grad(got, (x, wgu, wd))
+    assert torch.equal(got, want)
+    for a, b in zip(gg, gw):
+        assert torch.equal(a, b)
+
+
+def test_gradients_of_one_input(bcjr_mod):
+    """Gradients of the rows alone, of the weights alone, and none."""
+    g = gen(44)
+    off = torch.tensor([0, 5, 12], dtype=torch.int32, device=DEV)
+    x = torch.randn(12, 40, device=DEV, generator=g).half()
+    w = torch.randn(2, 24, 40, device=DEV, generator=g)
+    gy = torch.randn(12, 24, device=DEV, generator=g).half()
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    gx, gw = torch.autograd.grad(bcjr_mod.grouped_matmul(xr, wr, off), (xr, wr), gy)
+    assert torch.equal(torch.autograd.grad(bcjr_mod.grouped_matmul(xr, w, off), xr, gy)[0], gx)
+    assert torch.equal(torch.autograd.grad(bcjr_mod.grouped_matmul(x, wr, off), wr, gy)[0], gw)
+    assert not bcjr_mod.grouped_matmul(x, w, off).requires_grad
+
+
+@pytest.mark.parametrize("n,ld,dtype,to", [(1, 1, torch.float32, torch.bfloat16), (7, 9, torch.float32, torch.float16),
+                                           (8, 8, torch.float16, torch.float16), (517, 517, torch.bfloat16, torch.bfloat16),
+                                           (333, 340, torch.float16, torch.float16), (1024, 1024, torch.float32, torch.bfloat16)])
+def test_padded_copy(bcjr_mod, n, ld, dtype, to):
+    x = torch.randn(37, ld, device=DEV, generator=gen(n)).to(dtype)[:, :n]
+    out = bcjr_mod.moe._ops.pad_rows(x, torch.empty(0, device=DEV, dtype=to))
+    assert out.shape == x.shape and out.stride(0) == (n + 7) // 8 * 8 and torch.equal(out, x.to(to))
+    whole = torch.as_strided(out, (37, out.stride(0)), (out.stride(0), 1))
+    assert (whole[:, n:] == 0).all()

@@ -41,10 +41,10 @@ def test_route_refusals(lib, dtype, ld, T, E, k, status, msg):
 def test_route_workspace(lib):
     n = ctypes.c_size_t(7)
     assert lib.bcjr_moe_route_workspace(8, 64, ctypes.byref(n)) == 0 and n.value == 0
-    assert lib.bcjr_moe_route_workspace(16384, 64, ctypes.byref(n)) == 0 and n.value == 256 * 64 * 4
+    assert lib.bcjr_moe_route_workspace(16384, 64, ctypes.byref(n)) == 0 and n.value == 257 * 64 * 4
     assert lib.bcjr_moe_route_workspace(8, 64, None) == -1
-    assert lib.bcjr_moe_route(P, 0, 64, None, 16384, 64, 8, 0, P, P, P, P, P, P, 256 * 64 * 4 - 1, None) == -3
-    assert "65536 bytes" in _said(lib)
+    assert lib.bcjr_moe_route(P, 0, 64, None, 16384, 64, 8, 0, P, P, P, P, P, P, 257 * 64 * 4 - 1, None) == -3
+    assert "65792 bytes" in _said(lib)
     assert lib.bcjr_moe_route(P, 0, 64, None, 16384, 64, 8, 0, P, P, P, P, P, None, 1 << 20, None) == -1
     assert lib.bcjr_moe_route(None, 0, 64, None, 8, 64, 8, 0, P, P, P, P, P, None, 0, None) == -1
     assert "non-NULL" in _said(lib)
@@ -59,6 +59,8 @@ def test_route_workspace(lib):
     (1, 4, 1 << 31, 16, 16, -1, "M=2147483648"),
     (2, 4, 8, 0, 16, -1, "N=0"),
     (2, 4, 8, 16, 1 << 21, -1, "K=2097152"),
+    (1, 4, 1 << 30, 16, 16, -2, "more tiles"),
+    (1, 1024, 8, 1 << 20, 1 << 20, -2, "more tiles"),
 ])
 def test_grouped_refusals(lib, dtype, E, M, N, K, status, msg):
     assert lib.bcjr_grouped_matmul(P, dtype, K, M, None, P, K, 1, P, E, M, N, K, 0, P, None) == status
@@ -119,6 +121,7 @@ def test_combine_refusals(lib):
     (0, 32, float("inf"), 4, 32, 4, -1, "temperature"),
     (0, 32, 1e-45, 4, 32, 4, -1, "temperature"),
     (0, 32, 1.0, -1, 32, 4, -1, "T=-1"),
+    (0, 32, 1.0, 1 << 22, 32, 4, -2, "2^22"),
     (0, 32, 1.0, 4, 0, 0, -1, "V=0"),
     (0, 1 << 21, 1.0, 4, 1 << 21, 4, -2, "V=2097152"),
     (0, 32, 1.0, 4, 32, 33, -1, "K=33"),
