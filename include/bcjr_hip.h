@@ -323,6 +323,17 @@ int bcjr_grouped_matmul(const void* a, int dtype, int64_t lda, int64_t a_rows,
                         const int32_t* offsets, int64_t E, int64_t M, int64_t N, int64_t K,
                         int zero_padded, void* out, hipStream_t stream);
 
+/* bcjr_grouped_matmul with b_is_nk = 1 on float32 weights b, rounded to `dtype` (to
+ * nearest, ties to even) as they are read, without a copy of all of them: every
+ * expert's weights are read only if it has places.  b_copy (E, N, K) of `dtype`, or
+ * NULL, gets the rounded weights of the experts that have places (the others'
+ * stay as they are).  Rows in 16-byte chunks only: 16-byte aligned a and b, K and
+ * lda multiples of 8, ldb of 4; BCJR_EUNSUPPORTED otherwise. */
+int bcjr_grouped_matmul_f32w(const void* a, int dtype, int64_t lda, int64_t a_rows,
+                             const int32_t* rows, const float* b, int64_t ldb,
+                             const int32_t* offsets, int64_t E, int64_t M, int64_t N, int64_t K,
+                             void* out, void* b_copy, hipStream_t stream);
+
 /* Copies rows of n elements (dtype_in: F32 or `dtype`), ld apart, to rows ldo apart
  * (a multiple of 8, at least n) of dtype BF16 or F16, with zeros behind them; out
  * 16-byte aligned.  float32 is rounded to the nearest, ties to even. */

@@ -27,7 +27,7 @@ EXPORTS = (
     "bcjr_workspace_bytes", "bcjr_forward", "bcjr_forward_noalloc", "bcjr_forward_internals", "bcjr_forward_entropy", "bcjr_backward",
     "bcjr_viterbi", "bcjr_viterbi_constrained", "bcjr_viterbi_trace", "bcjr_decode", "bcjr_dequant", "bcjr_codebook", "bcjr_hadamard", "bcjr_rht", "bcjr_rht_batched",
     "bcjr_moe_route_workspace", "bcjr_moe_route", "bcjr_moe_route_backward", "bcjr_grouped_matmul",
-    "bcjr_grouped_wgrad", "bcjr_pad_rows", "bcjr_moe_combine", "bcjr_moe_combine_backward", "bcjr_topk_distill",
+    "bcjr_grouped_matmul_f32w", "bcjr_grouped_wgrad", "bcjr_pad_rows", "bcjr_moe_combine", "bcjr_moe_combine_backward", "bcjr_topk_distill",
     "bcjr_topk_distill_backward", "bcjr_topk_distill_both",
     "bcjr_strerror", "bcjr_last_error", "bcjr_version",
 )
@@ -124,6 +124,7 @@ def load(path: str = LIB_PATH):
     lib.bcjr_moe_route_backward.argtypes = [vp, i32, i64, vp, i64, i64, i32, i32, vp, vp, vp, vp, vp]
     lib.bcjr_grouped_matmul.argtypes = [vp, i32, i64, i64, vp, vp, i64, i32, vp, i64, i64, i64, i64, i32, vp, vp]
     lib.bcjr_grouped_wgrad.argtypes = [vp, i32, i64, vp, i64, i64, vp, vp, i64, i64, i64, i64, i32, i32, vp, vp]
+    lib.bcjr_grouped_matmul_f32w.argtypes = [vp, i32, i64, i64, vp, vp, i64, vp, i64, i64, i64, i64, vp, vp, vp]
     lib.bcjr_pad_rows.argtypes = [vp, i32, i64, i64, i64, i32, vp, i64, vp]
     lib.bcjr_moe_combine.argtypes = [vp, i32, i64, vp, vp, i64, i32, i64, i64, vp, vp]
     lib.bcjr_moe_combine_backward.argtypes = [vp, i32, i64, vp, vp, vp, vp, i64, i64, i32, i64, i64, vp, vp, vp]
@@ -134,7 +135,7 @@ def load(path: str = LIB_PATH):
     for name in ("bcjr_workspace_bytes", "bcjr_forward", "bcjr_forward_noalloc", "bcjr_forward_internals", "bcjr_forward_entropy",
                  "bcjr_backward", "bcjr_viterbi", "bcjr_viterbi_constrained", "bcjr_viterbi_trace", "bcjr_decode", "bcjr_dequant", "bcjr_codebook", "bcjr_hadamard", "bcjr_rht", "bcjr_rht_batched",
                  "bcjr_moe_route_workspace", "bcjr_moe_route", "bcjr_moe_route_backward", "bcjr_grouped_matmul",
-                 "bcjr_grouped_wgrad", "bcjr_pad_rows", "bcjr_moe_combine", "bcjr_moe_combine_backward", "bcjr_topk_distill",
+                 "bcjr_grouped_matmul_f32w", "bcjr_grouped_wgrad", "bcjr_pad_rows", "bcjr_moe_combine", "bcjr_moe_combine_backward", "bcjr_topk_distill",
                  "bcjr_topk_distill_backward", "bcjr_topk_distill_both"):
         getattr(lib, name).restype = i32
     for name in ("bcjr_strerror", "bcjr_last_error", "bcjr_version"):

@@ -68,8 +68,9 @@ def grouped_matmul(x, w, offsets, *, rows=None, slots=None):
 
     x:       (M, K) bfloat16 or float16 in sorted order or, with rows, (T, K):
              place p takes row rows[p] (a place outside [0, T) a row of zeros).
-    w:       (E, N, K), x's type or float32 (rounded to x's type for the
-             products; its gradient stays float32).
+    w:       (E, N, K), x's type or float32 (rounded to x's type as it is read;
+             its gradient stays float32).  A program that serves fixed
+             float32 weights rounds them once itself: half the bytes a call.
     offsets: (E + 1,) int32 on the device, ascending, from 0.
     rows, slots: of moe_route; slots (T, k), the places of each row, are needed
              for the gradient of a gathered x.

@@ -186,6 +186,26 @@ int bcjr_grouped_wgrad(const void* a, int dtype, int64_t lda, const void* b, int
   return launched(bcjr::launch_grouped_wgrad(P, dtype, out_f32 != 0, stream), "bcjr_grouped_wgrad launch");
 }
 
+int bcjr_grouped_matmul_f32w(const void* a, int dtype, int64_t lda, int64_t a_rows, const int32_t* rows,
+                             const float* b, int64_t ldb, const int32_t* offsets, int64_t E, int64_t M, int64_t N,
+                             int64_t K, void* out, void* b_copy, hipStream_t stream) {
+  if (int rc = check_grouped(dtype, E, M, N, K)) return rc;
+  if (a_rows < 0 || (!rows && a_rows < M))
+    return fail(BCJR_EINVAL, "a has %lld rows for M=%lld", (ll)a_rows, (ll)M);
+  if (a_rows > 1 && lda < K) return fail(BCJR_EINVAL, "row stride %lld is below K=%lld", (ll)lda, (ll)K);
+  if (ldb < K) return fail(BCJR_EINVAL, "row stride %lld of b is below %lld", (ll)ldb, (ll)K);
+  if (!bcjr::grouped_f32w_fits(a, lda, rows ? a_rows : 0, b, ldb, K) || (reinterpret_cast<uintptr_t>(b_copy) & 7))
+    return fail(BCJR_EUNSUPPORTED, "float32 weights need rows in 16-byte chunks: K=%lld, strides %lld, %lld", (ll)K,
+                (ll)lda, (ll)ldb);
+  if (M == 0) return BCJR_OK;
+  if ((!a && a_rows) || !b || !offsets || !out) return fail(BCJR_EINVAL, "a, b, offsets and out must be non-NULL");
+  bcjr::GroupedParams P = {};
+  P.a = a, P.b = b, P.rows = rows, P.offsets = offsets, P.out = out;
+  P.lda = lda, P.ldb = ldb, P.a_rows = a_rows, P.M = M, P.N = N, P.K = K, P.E = (int)E;
+  P.b_f32 = true, P.b_copy = b_copy;
+  return launched(bcjr::launch_grouped(P, dtype, true, stream), "bcjr_grouped_matmul_f32w launch");
+}
+
 int bcjr_pad_rows(const void* x, int dtype_in, int64_t ld, int64_t rows, int64_t n, int dtype, void* out, int64_t ldo,
                   hipStream_t stream) {
   if (int rc = check_dtype(dtype_in)) return rc;

@@ -248,12 +248,14 @@ __device__ __forceinline__ u16x8 fragment(const char* lds, int o, int ks) {
   }
 }
 
-enum { GM_NK, GM_KN, GM_WG };  // w (E, N, K); w (E, K, N); the weights' gradient
+// w (E, N, K); w (E, K, N); the weights' gradient; float32 w (E, N, K)
+enum { GM_NK, GM_KN, GM_WG, GM_NF };
 
 struct Place {
   int e;
   int64_t r0, r1;  // rows of the tile (products), of the group (weights' gradient)
   int64_t n0;
+  bool first;      // the first row tile of its group
 };
 
 // A value that all lanes have alike, in scalar registers.
@@ -328,6 +330,7 @@ __device__ __forceinline__ bool find_place(const int32_t* offsets, int E, int M,
       out->r0 = is_full ? ea + (int64_t)(local % en) * BM : ea + (int64_t)((eb - ea) / BM) * BM;
       out->r1 = is_full ? out->r0 + BM : eb;
       out->n0 = local / en;
+      out->first = out->r0 == ea;
       return true;
     }
     done += __shfl(upto, 63);
@@ -397,7 +400,7 @@ __device__ __forceinline__ void wave_fence() {
 
 template <class E, class O, int MODE, int BM, int BN>
 __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedParams P) {
-  constexpr bool ACOL = MODE == GM_WG, BCOL = MODE != GM_NK;
+  constexpr bool ACOL = MODE == GM_WG, BCOL = MODE == GM_KN || MODE == GM_WG, BF32 = MODE == GM_NF;
   constexpr int WM = 2, WN = 4;                             // waves along rows and columns
   static_assert(BM % 64 == 0 && BN % 64 == 0);
   constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;       // 16 x 16 blocks of a wave
@@ -429,7 +432,8 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
   auto b_chunk = [&](int r) { return lane % (64 / BR) ^ (BCOL ? col_swizzle<BN>(r) : (r >> 1) & 7); };
   const char* abase = (const char*)P.a;
   const char* bbase = (const char*)P.b;
-  if constexpr (MODE != GM_WG) bbase += (int64_t)t.e * (MODE == GM_NK ? P.N : P.K) * P.ldb * 2;
+  constexpr int kBSize = BF32 ? 4 : 2;
+  if constexpr (MODE != GM_WG) bbase += (int64_t)t.e * (BCOL ? P.K : P.N) * P.ldb * kBSize;
   uint32_t aoff[SA], boff[SB];
   if constexpr (!ACOL) {
     if (!P.rows) abase += m0 * P.lda * 2;
@@ -450,7 +454,9 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
       aoff[s] = m0 + c < mend ? (uint32_t)((r * P.lda + c) * 2) : kOutside;
     }
   }
-  if constexpr (!BCOL) {
+  if constexpr (BF32) {
+    bbase += n0 * P.ldb * 4;
+  } else if constexpr (!BCOL) {
     bbase += n0 * P.ldb * 2;
 #pragma unroll
     for (int s = 0; s < SB; ++s) {
@@ -488,13 +494,45 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
     for (int s = 0; s < SA; ++s)
       load_to_lds(pa, k0 + acut + (ACOL ? s * 8 * AR : 0) < K ? aoff[s] : kOutside, to + (s * 8 + wave) * 1024);
 #pragma unroll
-    for (int s = 0; s < SB; ++s) {
+    for (int s = 0; s < (BF32 ? 0 : SB); ++s) {
       uint32_t off = k0 + bcut + (BCOL ? s * 8 * BR : 0) < K ? boff[s] : kOutside;
       if constexpr (MODE == GM_WG)
         if (gather) off = off != kOutside && brow[s] < bmost ? off + brow[s] * (uint32_t)(P.ldb * 2) : kOutside;
       load_to_lds(pb, off, to + kABytes + (s * 8 + wave) * 1024);
     }
     if constexpr (MODE == GM_WG) find_rows(k0 + kBK);
+  };
+
+  // float32 weights go through registers: a step's 16-byte loads, 16 lanes a row,
+  // wait in `wide` for the next step, and are rounded on their way into LDS.  The
+  // first row tile of a group also leaves the rounded weights behind, if asked.
+  // (32,768 rows, 64 experts, 2048 x 2048: 496 us, with the copy 598; a copy first
+  // and then the product 274 + 343.  32 rows: 56, with the copy 119; 272 + 26.)
+  constexpr int SW = BF32 ? 2 * SB : 1;
+  u32x4 wide[SW];
+  const int wr = tid >> 4, wc = (tid & 15) * 4;  // row (32 more for each load), column
+  const bool leave = BF32 && P.b_copy && t.first;
+  auto load_wide = [&](int k0) {
+    const auto rb = __builtin_amdgcn_make_buffer_rsrc((void*)uniform((int64_t)(bbase + (int64_t)k0 * 4)), 0, 0xfffffff0u,
+                                                      0x00027000);
+#pragma unroll
+    for (int s = 0; s < SW; ++s) {
+      const int r = wr + 32 * s;
+      const uint32_t off = n0 + r < nend && k0 + wc < K ? (uint32_t)((r * P.ldb + wc) * 4) : kOutside;
+      wide[s] = __builtin_amdgcn_raw_buffer_load_b128(rb, off, 0, 0);
+    }
+  };
+  auto store_wide = [&](int k0, char* to) {
+#pragma unroll
+    for (int s = 0; s < SW; ++s) {
+      const int r = wr + 32 * s;
+      u16x4 v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = E::put(__uint_as_float(wide[s][i]));
+      *(u16x4*)(to + kABytes + row_at(r, wc >> 3) + (wc & 4) * 2) = v;
+      if (leave && n0 + r < nend && k0 + wc < K)
+        *(u16x4*)((uint16_t*)P.b_copy + ((int64_t)t.e * P.N + n0 + r) * P.K + k0 + wc) = v;
+    }
   };
 
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
@@ -504,12 +542,19 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
   if (steps) {
     if constexpr (MODE == GM_WG) find_rows(0);
     load(0, lds);
+    if constexpr (BF32) {
+      load_wide(0);
+      store_wide(0, lds);
+      load_wide(kBK);
+    }
   }
   for (int it = 0; it < steps; ++it) {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this step's tiles are in LDS
     __syncthreads();
     // past the end: zeros, where nothing is read
+    if constexpr (BF32) store_wide((it + 1) * kBK, lds + (~it & 1) * kBytes);
     load((it + 1) * kBK, lds + (~it & 1) * kBytes);
+    if constexpr (BF32) load_wide((it + 2) * kBK);
     if (!busy) continue;
     const char* from = lds + (it & 1) * kBytes;
     // MI groups of NJ matrix instructions for either half of the step; a group's
@@ -647,7 +692,14 @@ hipError_t launch_side(const GroupedParams& P, hipStream_t stream) {
 
 }  // namespace
 
+bool grouped_f32w_fits(const void* a, int64_t lda, int64_t gathered_rows, const void* b, int64_t ldb, int64_t K) {
+  return K % 8 == 0 && chunked(a, lda, gathered_rows > 256 ? gathered_rows : 256) &&
+         (reinterpret_cast<uintptr_t>(b) & 15) == 0 && ldb % 4 == 0 && 256 * ldb * 4 < (int64_t)0xfffffff0;
+}
+
 hipError_t launch_grouped(const GroupedParams& P, int dtype, bool b_is_nk, hipStream_t stream) {
+  if (P.b_f32)
+    return dtype == 1 ? launch_side<BF16, GM_NF, BF16>(P, stream) : launch_side<F16, GM_NF, F16>(P, stream);
   if ((P.zero_padded || (P.K % 8 == 0 && (b_is_nk || P.N % 8 == 0))) &&
       chunked(P.a, P.lda, P.rows ? P.a_rows : 256) && chunked(P.b, P.ldb, 256)) {
     if (dtype == 1)

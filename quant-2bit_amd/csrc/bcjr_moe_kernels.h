@@ -81,6 +81,10 @@ struct GroupedParams {
   int E;
   // zeros follow the rows of a and b up to a multiple of 8 elements
   bool zero_padded;
+  // b is float32 (E, N, K), rounded to a's type as it is read; b_copy (E, N, K), or
+  // null, gets the rounded weights of the experts that have rows
+  bool b_f32;
+  void* b_copy;
   int split;  // set by the launch
 };
 
@@ -107,6 +111,9 @@ hipError_t launch_combine(const CombineParams& P, int dtype, hipStream_t stream)
 hipError_t launch_combine_backward(const CombineBwdParams& P, int dtype, hipStream_t stream);
 // out (M, N) = a (M, K) times b (E, N, K) transposed (b_is_nk) or b (E, K, N).
 hipError_t launch_grouped(const GroupedParams& P, int dtype, bool b_is_nk, hipStream_t stream);
+// Whether the kernel on float32 weights takes these operands (gathered_rows: the
+// rows of a that places name, 0 if they are in order).
+bool grouped_f32w_fits(const void* a, int64_t lda, int64_t gathered_rows, const void* b, int64_t ldb, int64_t K);
 // out (E, N, K) = a^T b over each group's rows, a (M, N), b (M, K) (rows of b
 // through P.rows); out in float32 or the operands' type.
 hipError_t launch_grouped_wgrad(const GroupedParams& P, int dtype, bool out_f32, hipStream_t stream);

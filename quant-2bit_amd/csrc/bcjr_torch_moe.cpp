@@ -236,6 +236,37 @@ Tensor grouped_matmul_meta(const Tensor& x, const Tensor& w, const Tensor& offse
   return at::empty({p.M, p.N}, x.options());
 }
 
+// The product on float32 weights w (E, N, K), and the weights rounded to x's type
+// (of the experts that have places; empty without keep).
+std::tuple<Tensor, Tensor> grouped_f32w_hip(const Tensor& x_in, const Tensor& w_in, const Tensor& offsets_in,
+                                            const OptTensor& rows_in, bool keep) {
+  TORCH_CHECK(w_in.dim() == 3 && x_in.dim() == 2 && x_in.size(1) == w_in.size(2), "x must be (rows, K), w (E, N, K); got ",
+              x_in.sizes(), ", ", w_in.sizes());
+  TORCH_CHECK(w_in.scalar_type() == at::kFloat, "w must be float32; got ", w_in.scalar_type());
+  TORCH_CHECK(offsets_in.dim() == 1 && offsets_in.size(0) == w_in.size(0) + 1, "offsets must be (E+1=", w_in.size(0) + 1,
+              ",); got ", offsets_in.sizes());
+  same_device(x_in, w_in, "w");
+  same_device(x_in, offsets_in, "offsets");
+  same_device(x_in, rows_in, "rows");
+  const c10::OptionalDeviceGuard guard(at::device_of(x_in));
+  const Tensor x = strided_rows(x_in), w = w_in.contiguous(), offsets = as_int(offsets_in, "offsets");
+  const OptTensor rows = as_int(rows_in, "rows");
+  const int64_t E = w.size(0), N = w.size(1), K = w.size(2), M = rows ? rows->numel() : x.size(0);
+  Tensor out = at::empty({M, N}, x.options());
+  Tensor copy = keep ? at::empty({E, N, K}, x.options()) : at::empty({0}, x.options());
+  check(bcjr_grouped_matmul_f32w(x.data_ptr(), dtype_id(x, "x"), row_stride(x), x.size(0), iptr(rows),
+                                 w.data_ptr<float>(), K, offsets.data_ptr<int32_t>(), E, M, N, K, out.data_ptr(),
+                                 keep ? copy.data_ptr() : nullptr, stream_of(x)),
+        "bcjr_grouped_matmul_f32w");
+  return {out, copy};
+}
+
+std::tuple<Tensor, Tensor> grouped_f32w_meta(const Tensor& x, const Tensor& w, const Tensor& offsets,
+                                             const OptTensor& rows, bool keep) {
+  return {at::empty({rows ? rows->numel() : x.size(0), w.size(1)}, x.options()),
+          keep ? at::empty(w.sizes(), x.options()) : at::empty({0}, x.options())};
+}
+
 void wgrad_args(const Tensor& gy, const Tensor& x, const Tensor& offsets, const OptTensor& rows) {
   need_2d(gy, "gy");
   need_2d(x, "x");
@@ -292,6 +323,22 @@ Tensor call_pad(const Tensor& t, const Tensor& like) {
   return op.call(t, like);
 }
 
+std::tuple<Tensor, Tensor> call_f32w(const Tensor& x, const Tensor& w, const Tensor& offsets, const OptTensor& rows,
+                                     bool keep) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("bcjr::grouped_product_f32w", "")
+                       .typed<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
+                                                         bool)>();
+  return op.call(x, w, offsets, rows, keep);
+}
+
+// Whether the product reads float32 weights themselves: rows in 16-byte chunks, and
+// gathered rows within a buffer's reach.
+bool reads_f32(const Tensor& x, const Tensor& w) {
+  return w.scalar_type() == at::kFloat && x.scalar_type() != at::kFloat && x.size(1) % 8 == 0 && chunked(x) &&
+         w.is_contiguous() && w.storage_offset() % 4 == 0 && x.size(0) * x.stride(0) < (int64_t(1) << 31) - 16;
+}
+
 Tensor call_combine(const Tensor& y, const OptTensor& weights, const Tensor& slots);
 
 // t in `like`'s type with rows of 16-byte chunks: t itself, a converted copy or a padded one.
@@ -307,10 +354,15 @@ struct GroupedFunction : torch::autograd::Function<GroupedFunction> {
   static Variable forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& offsets,
                           const OptTensor& rows, const OptTensor& slots) {
     at::AutoDispatchBelowADInplaceOrView guard;
+    ctx->saved_data["w_f32"] = w.scalar_type() == at::kFloat;
+    if (reads_f32(x, w)) {
+      auto [y, wx] = call_f32w(x, w, offsets, rows, ctx->needs_input_grad(0));
+      ctx->save_for_backward({x, wx, offsets, rows ? *rows : Tensor(), slots ? *slots : Tensor()});
+      return y;
+    }
     // copies of float32 weights and of rows that are not 16-byte chunks serve the backward too
     const Tensor wx = in_chunks(w, x), xx = in_chunks(x, x);
     ctx->save_for_backward({xx, wx, offsets, rows ? *rows : Tensor(), slots ? *slots : Tensor()});
-    ctx->saved_data["w_f32"] = w.scalar_type() == at::kFloat;
     return call_grouped(xx, wx, offsets, rows, true, x.size(1) % 8 != 0);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -349,6 +401,7 @@ Tensor grouped_matmul(const Tensor& x, const Tensor& w, const Tensor& offsets, c
   const bool half = x.scalar_type() != at::kFloat;
   if (half && (wants_grad(x) || wants_grad(w))) return GroupedFunction::apply(x, w, offsets, rows, slots);
   at::AutoDispatchBelowADInplaceOrView guard;
+  if (reads_f32(x, w)) return std::get<0>(call_f32w(x, w, offsets, rows, false));
   const int64_t M = rows ? rows->numel() : x.size(0);
   // Rows that are not 16-byte chunks: a padded copy of all weights pays once the
   // experts have rows enough or the weights are small (or copied in any case);
@@ -590,6 +643,7 @@ TORCH_LIBRARY_FRAGMENT(bcjr, m) {
   m.def("grouped_product(Tensor x, Tensor w, Tensor offsets, Tensor? rows, bool w_is_nk, bool zero_padded=False) -> Tensor");
   m.def("grouped_wgrad(Tensor gy, Tensor x, Tensor offsets, Tensor? rows, bool zero_padded, bool out_f32) -> Tensor");
   m.def("pad_rows(Tensor x, Tensor like) -> Tensor");
+  m.def("grouped_product_f32w(Tensor x, Tensor w, Tensor offsets, Tensor? rows, bool keep) -> (Tensor, Tensor)");
   m.def("combine(Tensor y, Tensor? weights, Tensor slots) -> Tensor");
   m.def("combine_backward(Tensor y, Tensor weights, Tensor rows, Tensor slots, Tensor g_out) -> (Tensor, Tensor)");
   m.def("topk_distill(Tensor logits, Tensor values, Tensor indices, Tensor? teacher_lse, float temperature, bool keep) "
@@ -610,6 +664,7 @@ TORCH_LIBRARY_IMPL(bcjr, CUDA, m) {
   m.impl("grouped_product", &grouped_matmul_hip);
   m.impl("grouped_wgrad", &grouped_wgrad_hip);
   m.impl("pad_rows", &pad_rows_hip);
+  m.impl("grouped_product_f32w", &grouped_f32w_hip);
   m.impl("combine", &moe_combine_hip);
   m.impl("combine_backward", &moe_combine_backward_hip);
   m.impl("topk_distill", &topk_distill_hip);
@@ -623,6 +678,7 @@ TORCH_LIBRARY_IMPL(bcjr, Meta, m) {
   m.impl("grouped_product", &grouped_matmul_meta);
   m.impl("grouped_wgrad", &grouped_wgrad_meta);
   m.impl("pad_rows", &pad_rows_meta);
+  m.impl("grouped_product_f32w", &grouped_f32w_meta);
   m.impl("combine", &moe_combine_meta);
   m.impl("combine_backward", &moe_combine_backward_meta);
   m.impl("topk_distill", &topk_distill_meta);

@@ -89,6 +89,19 @@ def test_grouped_refuses_rows_and_strides(lib):
     assert lib.bcjr_grouped_wgrad(P, 1, 15, P, 16, 8, None, P, 4, 8, 15, 16, 1, 0, P, None) == -1
 
 
+def test_float32_weights_refusals(lib):
+    Q = ctypes.c_void_p(1 << 20)
+    assert lib.bcjr_grouped_matmul_f32w(P, 0, 16, 8, None, Q, 16, P, 4, 8, 16, 16, P, None, None) == -2
+    assert lib.bcjr_grouped_matmul_f32w(P, 1, 16, 7, None, Q, 16, P, 4, 8, 16, 16, P, None, None) == -1
+    for lda, ldb, K in [(16, 16, 12), (12, 16, 8), (16, 17, 16)]:
+        assert lib.bcjr_grouped_matmul_f32w(P, 1, lda, 8, None, Q, ldb, P, 4, 8, 16, K, P, None, None) == -2
+        assert "16-byte chunks" in _said(lib)
+    assert lib.bcjr_grouped_matmul_f32w(P, 1, 16, 8, None, ctypes.c_void_p(4100), 16, P, 4, 8, 16, 16, P, None, None) == -2
+    assert lib.bcjr_grouped_matmul_f32w(P, 1, 16, 8, None, Q, 16, P, 4, 8, 16, 16, P, ctypes.c_void_p(4100), None) == -2
+    assert lib.bcjr_grouped_matmul_f32w(P, 1, 16, 8, None, Q, 15, P, 4, 8, 16, 16, P, None, None) == -1
+    assert lib.bcjr_grouped_matmul_f32w(None, 1, 16, 0, None, None, 16, None, 4, 0, 16, 16, None, None, None) == 0
+
+
 def test_pad_rows_refusals(lib):
     assert lib.bcjr_pad_rows(P, 0, 16, 4, 16, 0, P, 16, None) == -2
     assert lib.bcjr_pad_rows(P, 2, 16, 4, 16, 1, P, 16, None) == -2
@@ -166,6 +179,7 @@ def test_meta_shapes():
     W = torch.empty(6, 24, 16, device="meta", requires_grad=True)
     y = ops.grouped_matmul(x, W, o, r, s)
     assert y.shape == (30, 24) and y.dtype == torch.bfloat16
+    assert ops.pad_rows(torch.empty(3, 5, device="meta"), l).stride() == (8, 1)
     gx, gw = torch.autograd.grad(y, (x, W), torch.empty_like(y))
     assert gx.shape == x.shape and gx.dtype == x.dtype and gw.shape == W.shape and gw.dtype == torch.float32
     wr = torch.empty(10, 3, device="meta", requires_grad=True)
