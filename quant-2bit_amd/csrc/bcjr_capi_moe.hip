@@ -104,7 +104,11 @@ bcjr::DistillParams distill_params(const void* logits, int64_t ld, const float* 
   P.ld = T > 1 ? ld : V;
   P.V = (int)V;
   P.K = (int)K;
-  P.inv_tau = 1.f / temperature;
+  P.inv_tau = 1. / (double)temperature;
+  const double scale = 1.4426950408889634 * P.inv_tau;
+  P.scale_hi = (float)scale;
+  if ((double)P.scale_hi >= scale) P.scale_hi = std::nextafterf(P.scale_hi, 0.f);
+  P.scale_lo = (float)(scale - (double)P.scale_hi);
   return P;
 }
 

@@ -16,9 +16,13 @@
 // share of the loss needs the student's normaliser only as a factor.  The
 // gradient reads the row again and writes it once, and overwrites the K entries
 // behind a barrier; where loss and gradient are one call, a thread keeps its
-// first C vectors of the row in registers between the two.  Exponents are base 2
-// and of differences from the row's maximum m; sums are float32.
-// stats[row] = (m, log2 of the sum, c, c - r / p_r, n in log2 units, 3 unused).
+// first C vectors of the row in registers between the two.
+//
+// Exponents are of differences from the row's maximum m, which are exact or nearly
+// so; log2(e) / tau is held in two floats, since the rounding of one would move
+// all terms the same way.  The row's sums are float32.  What is done K times or
+// once a row is done in 64 bits: a divergence is a small difference of logarithms.
+// stats[row] = (m, 1 / the sum, c, c - r / p_r; n as a double, 2 unused).
 #include "bcjr_moe_device.h"
 #include "bcjr_moe_kernels.h"
 
@@ -27,22 +31,26 @@ namespace bcjr {
 namespace {
 
 constexpr int kUnroll = 4;  // vectors in flight per thread beside the kept ones
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // A teacher's mass outside its entries below this is what float32 sums leave of
 // 1 by rounding: none.
-constexpr float kRest = 1e-6f;
+constexpr double kRest = 1e-6;
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float lg2(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.f : m; }
+
+// 2^(d log2(e) / tau); lo > 0, so that -inf stays -inf.
+struct Scale {
+  float hi, lo;
+  __device__ __forceinline__ float exp(float d) const { return ex2(fmaf(d, lo, d * hi)); }
+};
 
 // Running maximum of logits, and sums of exponentials over it: all, and those
 // outside the entries.
 struct Run {
   float m = -INFINITY, l = 0.f, r = 0.f;
-  __device__ __forceinline__ void raise(float to, float s2) {
+  __device__ __forceinline__ void raise(float to, Scale s2) {
     if (to > m) {
-      const float f = ex2((m - to) * s2);  // 0 the first time
+      const float f = s2.exp(m - to);  // 0 the first time
       l *= f;
       r *= f;
       m = to;
@@ -50,12 +58,19 @@ struct Run {
   }
 };
 
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
 template <class E, int KIND, bool VEC, int NT, int C>
 __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParams P) {
   constexpr int N = VEC ? Vec16<E>::N : 1, NW = NT / 64;
   using raw = typename E::raw;
   extern __shared__ __align__(16) uint32_t marked[];  // one bit per element, from `lead` on
-  __shared__ float top[NW], part[2][NW], teacher[4];
+  __shared__ float top[NW], part[2][NW];
+  __shared__ double teacher[4];
   __shared__ int repeated;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
@@ -63,7 +78,7 @@ __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParam
   raw* g = KIND == DISTILL_LOSS ? nullptr : (raw*)P.grad + row * P.V;
   const float* tv = P.values + row * P.K;
   const int32_t* ti = P.indices + row * P.K;
-  const float s2 = P.inv_tau * kLog2e;  // logits to log2 units
+  const Scale s2 = {P.scale_hi, P.scale_lo};
   const bool rest = KIND != DISTILL_BACKWARD && P.teacher_lse != nullptr;
   // elements of the row's first 16-byte block that lie before the row
   const int lead = VEC ? (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(raw)) : 0;
@@ -88,13 +103,14 @@ __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParam
     __syncthreads();
   }
 
-  float m, L, c, outside, n2;  // m as it is subtracted
+  float m, inv, c, outside;  // m as it is subtracted
+  double n;
   u32x4 keep[C > 0 ? C : 1];
   auto vector_at = [&](int v) { return *(const u32x4*)(xv + (int64_t)v * N); };
   if constexpr (KIND == DISTILL_BACKWARD) {
     const float4 s = P.stats[2 * row];
-    m = s.x, L = s.y, c = s.z, outside = s.w;
-    n2 = P.stats[2 * row + 1].x;
+    m = s.x, inv = s.y, c = s.z, outside = s.w;
+    n = *(const double*)&P.stats[2 * row + 1];
   } else {
     Run a;
     // exponentials over a vector, and the same without the entries
@@ -102,7 +118,7 @@ __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParam
       const float ref = finite_or_0(a.m);
       float e[N], s = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) s += e[i] = ex2((z[i] - ref) * s2);
+      for (int i = 0; i < N; ++i) s += e[i] = s2.exp(z[i] - ref);
       a.l += s;
       if (rest) {
         const uint32_t bits = (marked[(v * N) >> 5] >> ((v * N) & 31)) & ((1u << N) - 1);
@@ -170,35 +186,36 @@ __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParam
       take(z, edge);
     }
 
-    // The entries, by one wave: n2, sum q, the largest student logit x_k among
-    // them and sum q (log q - (x - x_k)).
+    // The entries, by one wave: n, sum q, the largest student logit x_k among
+    // them and sum q (log q - (x - x_k) / tau).
     if (wave == NW - 1) {
       float most = -INFINITY;
       if (rest) {
-        n2 = P.teacher_lse[row] * kLog2e;
+        n = P.teacher_lse[row];
       } else {
-        float l = 0.f;
+        double l = 0.;
         for (int k = lane; k < P.K; k += 64)
           if (entry(k)) most = fmaxf(most, tv[k]);
-        const float ref = finite_or_0(wave_max(most));
+        const double ref = finite_or_0(wave_max(most));
         for (int k = lane; k < P.K; k += 64)
-          if (entry(k)) l += ex2((tv[k] - ref) * s2);
-        n2 = ref * s2 + lg2(wave_sum(l));  // -inf for a row without entries
+          if (entry(k)) l += expf((float)((tv[k] - ref) * P.inv_tau));
+        n = ref * P.inv_tau + log(wave_sum(l));  // -inf for a row without entries
       }
       most = -INFINITY;
       for (int k = lane; k < P.K; k += 64)
         if (entry(k)) most = fmaxf(most, E::get(x[ti[k]]));
-      const float xk = finite_or_0(wave_max(most));
-      float mass = 0.f, term = 0.f;
+      const double xk = finite_or_0(wave_max(most));
+      double mass = 0., term = 0.;
       for (int k = lane; k < P.K; k += 64)
         if (entry(k)) {
-          const float lq = tv[k] * s2 - n2, q = ex2(lq);
+          const double lq = tv[k] * P.inv_tau - n;
+          const float q = expf((float)lq);
           mass += q;
-          if (q != 0.f) term += q * (lq - (E::get(x[ti[k]]) - xk) * s2);
+          if (q != 0.f) term += q * (lq - (E::get(x[ti[k]]) - xk) * P.inv_tau);
         }
       mass = wave_sum(mass);
       term = wave_sum(term);
-      if (lane == 0) teacher[0] = n2, teacher[1] = mass, teacher[2] = term, teacher[3] = xk;
+      if (lane == 0) teacher[0] = n, teacher[1] = mass, teacher[2] = term, teacher[3] = xk;
     }
     const float wm = wave_max(a.m);
     if (lane == 0) top[wave] = wm;
@@ -207,7 +224,7 @@ __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParam
 #pragma unroll
     for (int i = 1; i < NW; ++i) m = fmaxf(m, top[i]);
     m = finite_or_0(m);
-    const float f = a.m == -INFINITY ? 1.f : ex2((a.m - m) * s2);
+    const float f = a.m == -INFINITY ? 1.f : s2.exp(a.m - m);
     const float wl = wave_sum(a.l * f), wr = rest ? wave_sum(a.r * f) : 0.f;
     if (lane == 0) part[0][wave] = wl, part[1][wave] = wr;
     __syncthreads();
@@ -217,39 +234,39 @@ __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParam
       total += part[0][i];
       if (rest) others += part[1][i];
     }
-    L = lg2(total);
-    n2 = teacher[0];
-    const float mass = teacher[1];
-    float loss = mass == 0.f ? 0.f : (teacher[2] + mass * ((m - teacher[3]) * s2 + L)) * kLn2;
-    outside = c = rest ? mass : (n2 == -INFINITY ? 0.f : 1.f);
+    inv = 1.f / total;
+    n = teacher[0];
+    const double mass = teacher[1];
+    double r = 0.;
+    const float pr = others / total;
     if (rest) {
-      const float pr = others / total;
-      float r = 1.f - mass;
-      r = r > kRest ? r : 0.f;
-      c = mass + r;
-      outside = c;
-      if (r > 0.f) {
-        loss += r * (lg2(r) - lg2(pr)) * kLn2;
-        if (pr > 0.f) outside = c - r / pr;
-      }
+      r = 1. - mass;
+      if (!(r > kRest)) r = 0.;
+      outside = c = (float)(mass + r);
+      if (r > 0. && pr > 0.f) outside = c - (float)r / pr;
+    } else {
+      outside = c = n == -INFINITY ? 0.f : 1.f;
     }
-    if (c == 0.f) loss = 0.f;  // no entries
     if (tid == 0) {
-      P.loss[row] = loss;
+      double loss = mass == 0. ? 0. : teacher[2] + mass * ((m - teacher[3]) * P.inv_tau + log((double)total));
+      if (r > 0.) loss += r * (log(r) - log((double)pr));
+      if (c == 0.f) loss = 0.;  // no entries
+      P.loss[row] = (float)loss;
       if (P.stats) {
-        P.stats[2 * row] = make_float4(m, L, c, outside);
-        P.stats[2 * row + 1] = make_float4(n2, 0.f, 0.f, 0.f);
+        P.stats[2 * row] = make_float4(m, inv, c, outside);
+        *(double2*)&P.stats[2 * row + 1] = make_double2(n, 0.);
       }
     }
   }
 
   if constexpr (KIND != DISTILL_LOSS) {
-    const float scale = P.g_rows[row] * P.inv_tau;
+    const float scale = (float)(P.g_rows[row] * P.inv_tau);
     // rows that count nothing: zeros, whatever their logits are
     const bool none = scale == 0.f || c == 0.f;
-    const float go = scale * outside;
-    auto p_of = [&](float z) { return ex2(fmaf(z - m, s2, -L)); };
-    auto out = [&](float z) { return none ? 0.f : p_of(z) * go; };
+    const float go = scale * outside * inv;
+    
+    auto q_of = [&](int k) { return expf((float)(tv[k] * P.inv_tau - n)); };
+    auto out = [&](float z) { return none ? 0.f : s2.exp(z - m) * go; };
     auto write = [&](int v, u32x4 t) {
       float z[N];
       unpack16<E>(t, z);
@@ -288,12 +305,12 @@ __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParam
       const int i = ti[k];
       float q = 0.f;
       if (!repeated) {
-        q = ex2(tv[k] * s2 - n2);
+        q = q_of(k);
       } else {
         for (int o = 0; o < P.K; ++o)
-          if (ti[o] == i) q += ex2(tv[o] * s2 - n2);
+          if (ti[o] == i) q += q_of(o);
       }
-      g[i] = E::put(scale * (p_of(E::get(x[i])) * c - q));
+      g[i] = E::put(scale * (s2.exp(E::get(x[i]) - m) * inv * c - q));
     }
   }
 }

@@ -99,7 +99,8 @@ struct DistillParams {
   void* grad;               // (T, V)
   int64_t T, ld;
   int V, K;
-  float inv_tau;
+  double inv_tau;
+  float scale_hi, scale_lo;  // log2(e) / tau in two parts, the second above 0
 };
 
 // Stores `text` for bcjr_last_error() and returns the status (bcjr_capi.hip).
