@@ -320,12 +320,13 @@ __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParam
 // workgroups let rows overlap their beginnings and ends; large ones keep more of a
 // long row on the chip between its two uses.  Loss with gradient, microseconds,
 // 256 threads keeping 12 vectors / 512 keeping 16 / 1,024 keeping 16:
-//   8,192 rows of  8,000 float32  (2,000 vectors)   105 /  143 /  234
-//   1,024 rows of 32,000 bfloat16 (4,000)            30 /   33 /   44
-//   4,096 rows of 50,257 bfloat16 (6,282)           214 /  197 /  237
-//   8,192 rows of 131,072 bfloat16 (16,384)       1,211 /  981 / 1,022
-//   4,096 rows of 131,072 float32 (32,768)        1,217 / 1,114 /  913
-// (keeping none: 140, 34, 218, 1,055 and 1,166 at the best width of each).
+//   8,192 rows of  8,000 float32  (2,000 vectors)   110 /  157 /  263
+//   1,024 rows of 32,000 bfloat16 (4,000)            32 /   36 /   50
+//     256 rows of 32,000 bfloat16 (4,000)            18 /   14 /   14
+//   4,096 rows of 50,257 bfloat16 (6,282)           217 /  207 /  255
+//   8,192 rows of 131,072 bfloat16 (16,384)       1,215 /  986 / 1,076
+//   4,096 rows of 131,072 float32 (32,768)        1,212 / 1,112 /  920
+// (Keeping none cost 140, 34, 14, 218, 1,055 and 1,166 at the best width of each.)
 int row_threads(int64_t nvec) { return nvec < 3000 ? 256 : nvec <= 16384 ? 512 : 1024; }
 
 template <class E>
