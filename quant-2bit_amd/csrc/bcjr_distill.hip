@@ -264,7 +264,7 @@ __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParam
     // rows that count nothing: zeros, whatever their logits are
     const bool none = scale == 0.f || c == 0.f;
     const float go = scale * outside * inv;
-    
+
     auto q_of = [&](int k) { return expf((float)(tv[k] * P.inv_tau - n)); };
     auto out = [&](float z) { return none ? 0.f : s2.exp(z - m) * go; };
     auto write = [&](int v, u32x4 t) {

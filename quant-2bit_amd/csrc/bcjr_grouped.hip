@@ -378,14 +378,16 @@ constexpr uint32_t kOutside = 0xffffffffu;  // a buffer offset that loads zeros
 // Loads 16 bytes a lane from `base` + off into the KiB of LDS at `to` (uniform),
 // in lane order; no register receives data.  Written as an instruction because
 // the compiler lets the transposing LDS reads of the other buffer wait for every
-// such load that it sees.  Whoever reads the KiB waits for vmcnt first.
+// such load that it sees.  Whoever reads the KiB waits for vmcnt first.  Five
+// wait states stand between a vector instruction that wrote a scalar of the
+// descriptor and the load that reads it: the compiler counts none inside asm.
 __device__ __forceinline__ void load_to_lds(const char* base, uint32_t off, char* to) {
   const uint64_t b = (uint64_t)uniform((int64_t)base);
   const u32x4 desc = {(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, 0xfffffff0u, 0x00027000u};
   const uint32_t at = (uint32_t)uniform((int)(uint32_t)(uintptr_t)(lds_char*)to);
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
+      "s_nop 3\n\t"
       "buffer_load_dwordx4 %1, %2, 0 offen lds"
       ::"s"(at), "v"(off), "s"(desc)
       : "memory", "m0");
