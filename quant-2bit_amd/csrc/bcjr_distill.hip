@@ -23,6 +23,12 @@
 // all terms the same way.  The row's sums are float32.  What is done K times or
 // once a row is done in 64 bits: a divergence is a small difference of logarithms.
 // stats[row] = (m, 1 / the sum, c, c - r / p_r; n as a double, 2 unused).
+//
+// Bound by the logits' bytes, at a copy's rate: 4,096 rows of 50,257 bfloat16, 64
+// entries, take 83 us (loss, 4.9 TB/s) and 173 (gradient, 4.75), together in one call
+// 210 (3.9 of one read and one write: part of a row is read twice, and neither the
+// loads nor the stores overlap the other half of the same row).  8,192 rows of
+// 131,072 take 389 (5.5), 845 (5.1) and 980 (4.4).
 #include "bcjr_moe_device.h"
 #include "bcjr_moe_kernels.h"
 

@@ -84,7 +84,9 @@ int64_t max_tiles(int64_t M, int64_t E, int BM) {
 //
 // 64 x 64 tiles of the output, 32 of the reduction at a time, element loads
 // with bounds into LDS: for row lengths and strides that 16-byte loads cannot
-// take.  Four waves, 32 x 32 outputs each.
+// take.  Four waves, 32 x 32 outputs each.  Bound by its two-byte loads: 512 rows
+// on 64 experts of 1023 x 2047 take 145 us, 1.9 TB/s of the weights, and 2,048 rows
+// 253, 34 TFLOP/s; what calls it first weighs a padded copy against that.
 constexpr int kT = 64, kTk = 32, kPad = kTk + 8;
 
 template <class E>
@@ -213,7 +215,17 @@ __global__ __launch_bounds__(256) void wgrad_any_kernel(GroupedParams P) {
 // as [64][column], read with the transposing LDS read: 16 lanes take a 4 x 16
 // block, each ends with one column's four values.  The 16-byte chunks of a row
 // are permuted by its number so that the 16 lanes of a read's pass meet
-// distinct banks.
+// distinct banks (counted conflicts: none).
+//
+// With many rows the matrix instructions bind, at the clock that the card's power
+// allows under them: 64 groups of 512 rows, 2048 x 2048, take 245 us forward, 1.12
+// PFLOP/s (a library's product of 8192 cubed 1.32), 1.75 GHz with the matrix units
+// busy 56 % of the time; uneven groups add short tiles and a longer last round (0.75).
+// The weights' gradient, 465 us, also writes E N K values in float32.  With few
+// rows the weights' bytes bind: 32 rows on about 26 of 64 experts take 45 us, 4.9 TB/s.
+// Side by side on the large products, 256 x 256 tiles beat 128 x 256 and 128 x 128
+// (less data moved per instruction), and two buffers of 64 beat three to five of 32
+// (64-byte pieces of rows).
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBK = 64;
@@ -375,23 +387,33 @@ typedef __attribute__((address_space(3))) char lds_char;
 constexpr int kAhead = 2;  // groups of matrix instructions that a fragment is read ahead
 constexpr uint32_t kOutside = 0xffffffffu;  // a buffer offset that loads zeros
 
-// Loads 16 bytes a lane from `base` + off into the KiB of LDS at `to` (uniform),
-// in lane order; no register receives data.  Written as an instruction because
-// the compiler lets the transposing LDS reads of the other buffer wait for every
-// such load that it sees.  Whoever reads the KiB waits for vmcnt first.  Five
-// wait states stand between a vector instruction that wrote a scalar of the
-// descriptor and the load that reads it: the compiler counts none inside asm.
-__device__ __forceinline__ void load_to_lds(const char* base, uint32_t off, char* to) {
+// S times: loads 16 bytes a lane from `base` + off[s] into the KiB of LDS at `to`
+// (uniform) + 8 KiB s, in lane order; no register receives data.  Written as
+// instructions because the compiler lets the transposing LDS reads of the other
+// buffer wait for every such load that it sees.  Whoever reads the LDS waits for
+// vmcnt first.  Five wait states stand between a vector instruction that wrote a
+// scalar of the descriptor and the load that reads it, one after m0 is written: the
+// compiler counts none inside asm.
+#define BCJR_NEXT_KIB(off) "\n\ts_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tbuffer_load_dwordx4 " off ", %1, 0 offen lds"
+template <int S>
+__device__ __forceinline__ void load_to_lds(const char* base, const uint32_t (&off)[S], char* to) {
+  static_assert(S == 1 || S == 2 || S == 4);
   const uint64_t b = (uint64_t)uniform((int64_t)base);
   const u32x4 desc = {(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, 0xfffffff0u, 0x00027000u};
   const uint32_t at = (uint32_t)uniform((int)(uint32_t)(uintptr_t)(lds_char*)to);
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 3\n\t"
-      "buffer_load_dwordx4 %1, %2, 0 offen lds"
-      ::"s"(at), "v"(off), "s"(desc)
-      : "memory", "m0");
+#define BCJR_FIRST_KIB "s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %2, %1, 0 offen lds"
+  if constexpr (S == 1)
+    asm volatile(BCJR_FIRST_KIB ::"s"(at), "s"(desc), "v"(off[0]) : "memory", "m0");
+  else if constexpr (S == 2)
+    asm volatile(BCJR_FIRST_KIB BCJR_NEXT_KIB("%3")::"s"(at), "s"(desc), "v"(off[0]), "v"(off[1])
+                 : "memory", "m0", "scc");
+  else
+    asm volatile(BCJR_FIRST_KIB BCJR_NEXT_KIB("%3") BCJR_NEXT_KIB("%4") BCJR_NEXT_KIB("%5")::"s"(at), "s"(desc),
+                 "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3])
+                 : "memory", "m0", "scc");
+#undef BCJR_FIRST_KIB
 }
+#undef BCJR_NEXT_KIB
 
 // LDS of a wave: what its lanes wrote before, all of them read after.  (The LDS
 // works off a wave's instructions in order: only the compiler has to keep them.)
@@ -492,15 +514,19 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
   auto load = [&](int k0, char* to) {
     const char* pa = abase + (ACOL ? k0 * P.lda : (int64_t)k0) * 2;
     const char* pb = bbase + (gather ? 0 : BCOL ? k0 * P.ldb : (int64_t)k0) * 2;
+    uint32_t oa[SA];
 #pragma unroll
-    for (int s = 0; s < SA; ++s)
-      load_to_lds(pa, k0 + acut + (ACOL ? s * 8 * AR : 0) < K ? aoff[s] : kOutside, to + (s * 8 + wave) * 1024);
+    for (int s = 0; s < SA; ++s) oa[s] = k0 + acut + (ACOL ? s * 8 * AR : 0) < K ? aoff[s] : kOutside;
+    load_to_lds(pa, oa, to + wave * 1024);
+    if constexpr (!BF32) {
+      uint32_t ob[SB];
 #pragma unroll
-    for (int s = 0; s < (BF32 ? 0 : SB); ++s) {
-      uint32_t off = k0 + bcut + (BCOL ? s * 8 * BR : 0) < K ? boff[s] : kOutside;
-      if constexpr (MODE == GM_WG)
-        if (gather) off = off != kOutside && brow[s] < bmost ? off + brow[s] * (uint32_t)(P.ldb * 2) : kOutside;
-      load_to_lds(pb, off, to + kABytes + (s * 8 + wave) * 1024);
+      for (int s = 0; s < SB; ++s) {
+        ob[s] = k0 + bcut + (BCOL ? s * 8 * BR : 0) < K ? boff[s] : kOutside;
+        if constexpr (MODE == GM_WG)
+          if (gather) ob[s] = ob[s] != kOutside && brow[s] < bmost ? ob[s] + brow[s] * (uint32_t)(P.ldb * 2) : kOutside;
+      }
+      load_to_lds(pb, ob, to + kABytes + wave * 1024);
     }
     if constexpr (MODE == GM_WG) find_rows(k0 + kBK);
   };
@@ -660,19 +686,20 @@ bool chunked(const void* p, int64_t ld, int64_t rows) {
 
 // Side of the square output tiles.  Larger tiles load less for the same work and
 // smaller ones leave fewer compute units idle; the counts below take every group
-// to have a short tile.  Measured (microseconds at 256 / 128 / 64, bfloat16):
-//   products  4096 tokens x 8, 64 experts, 2048 x 2048 (1,536 tiles of 256)  410 / 476 / -
-//             1024 x 8, 64, 2048 x 2048 (768)       178 / 178 / 215
-//             256 x 8, 64, 2048 x 2048 (576)        127 / 120 / -
-//             2048 x 4, 64, 1024 x 1024 (384)        53 /  40 /  54
-//             1024 x 2, 8, 1024 x 1024 (192 of 128)  34 /  16 /  19
-//             512 rows on 8, 512 x 512 (60 of 128)   22 /  10 /   7
+// to have a short tile.  Measured (microseconds at 256 / 128 / 64, bfloat16, the
+// groups as a router with favourites fills them):
+//   products  4096 tokens x 8, 64 experts, 2048 x 2048 (1,536 tiles of 256)  351 / 399 / 620
+//             1024 x 8, 64, 2048 x 2048 (768)       166 / 181 / 220
+//             256 x 8, 64, 2048 x 2048 (576)        125 / 120 / 132
+//             2048 x 4, 64, 1024 x 1024 (384)        57 /  46 /  61
+//             1024 x 2, 8, 1024 x 1024 (192 of 128)  29 /  15 /  16
+//             256 x 2, 8, 512 x 512 (48 of 128)      16 / 8.6 / 6.4
 //   and of a few rows, where the weights' bytes count and not the row tiles:
-//             4 tokens x 8, 64, 2048 x 2048 (512 of 128)  34 / 26 / 26
-//             8 x 2, 8, 4096 x 4096 (256 of 128)          57 / 39 / 32
-//   weights' gradient  8 experts, 2048 x 2048 (512)    25 / 29 / 44
-//             16, 1024 x 1024 (256; 1,024 of 128)      22 / 21 / 31
-//             4, 512 x 2048 (256 of 128)               64 / 28 / 21
+//             4 tokens x 8, 64, 2048 x 2048 (512 of 128)  51 / 46 / 44
+//             8 x 2, 8, 4096 x 4096 (256 of 128)          79 / 60 / 53
+//   weights' gradient  2048 x 2 on 8 experts, 2048 x 2048 (512)  56 / 57 / 92
+//             2048 x 2 on 16, 1024 x 1024 (256; 1,024 of 128)    50 / 26 / 38
+//             2048 on 4, 512 x 2048 (64; 256 of 128)             45 / 20 / 17
 int product_side(const GroupedParams& P) {
   const int64_t groups = P.E < P.M ? P.E : P.M;
   auto tiles = [&](int64_t s) { return (P.M / s + groups) * ((P.N + s - 1) / s); };
