@@ -298,7 +298,7 @@ int bcjr_moe_route(const void* logits, int dtype, int64_t ld, const uint8_t* val
                    hipStream_t stream);
 
 /* g_logits (T, E) of `dtype` from g_weights (T, k) and the outputs of
- * bcjr_moe_route; the choice of experts has no gradient. */
+ * bcjr_moe_route; the choice of experts has no gradient.  T < 2^26. */
 int bcjr_moe_route_backward(const void* logits, int dtype, int64_t ld, const uint8_t* valid,
                             int64_t T, int64_t E, int k, int renormalize, const float* weights,
                             const int32_t* experts, const float* g_weights, void* g_logits,
@@ -312,7 +312,7 @@ int bcjr_moe_route_backward(const void* logits, int dtype, int64_t ld, const uin
  *   b_is_nk = 1: b (E, N, K), out = a b^T (weights as a linear layer holds them)
  *   b_is_nk = 0: b (E, K, N), out = a b
  * with row stride ldb, the matrices of b back to back.
- * BF16 or F16, products summed in float32.  E <= 1024; M < 2^31.
+ * BF16 or F16, products summed in float32.  E <= 1024; M < 2^30 - 2^17; N, K <= 2^20.
  * Rows in 16-byte chunks (16-byte aligned bases, strides and K, for b_is_nk = 0 N
  * too, multiples of 8) take the fast kernel, others one that is many times
  * slower.  zero_padded = 1 says that the rows of a and b lie 8 elements apart or a

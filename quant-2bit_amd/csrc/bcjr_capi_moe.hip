@@ -62,9 +62,10 @@ int check_grouped(int dtype, int64_t E, int64_t M, int64_t N, int64_t K) {
   if (M < 0 || M > INT32_MAX) return fail(BCJR_EINVAL, "M=%lld rows outside [0, 2^31)", (ll)M);
   if (N < 1 || N > kMaxDim || K < 1 || K > kMaxDim)
     return fail(BCJR_EINVAL, "N=%lld, K=%lld must be in [1, %lld]", (ll)N, (ll)K, (ll)kMaxDim);
-  // a launch has fewer than 2^32 threads, 512 a tile of 256 x 256
-  const int64_t most = 1 << 23, n = N / 256 + 1, k = K / 256 + 1;
-  if ((M / 256 + E + 1) * (n > k ? n : k) >= most || E * n * k >= most || M >= 1 << 30)
+  // A launch has fewer than 2^32 threads a dimension: 512 a tile of 256 x 256, a few
+  // more for the eight dies' equal shares, 256 a row tile of 64 in the slow kernel.
+  const int64_t most = (1 << 23) - 16, n = N / 256 + 1, k = K / 256 + 1;
+  if ((M / 256 + E + 1) * (n > k ? n : k) >= most || E * (n + 7) * (k + 7) >= most || M >= (1 << 30) - (1 << 17))
     return fail(BCJR_EUNSUPPORTED, "M=%lld, N=%lld, K=%lld, E=%lld: more tiles than a launch holds", (ll)M, (ll)N, (ll)K,
                 (ll)E);
   return BCJR_OK;
@@ -145,6 +146,8 @@ int bcjr_moe_route_backward(const void* logits, int dtype, int64_t ld, const uin
   if (T == 0) return BCJR_OK;
   if (!logits || !weights || !experts || !g_weights || !g_logits)
     return fail(BCJR_EINVAL, "logits, weights, experts, g_weights and g_logits must be non-NULL");
+  if (T >= 1 << 26)
+    return fail(BCJR_EUNSUPPORTED, "T=%lld tokens: the routing's gradient is built for fewer than 2^26", (ll)T);
   const bcjr::RouteBwdParams P = {logits, valid, weights, experts, g_weights, g_logits,
                                   T,      ld,    (int)E,  k,       renormalize ? 1 : 0};
   return launched(bcjr::launch_route_backward(P, dtype, stream), "bcjr_moe_route_backward launch");

@@ -38,6 +38,22 @@ def test_route_refusals(lib, dtype, ld, T, E, k, status, msg):
     assert msg in _said(lib)
 
 
+def test_route_gradient_refuses_more_tokens_than_a_launch_holds(lib):
+    assert lib.bcjr_moe_route_backward(P, 0, 8, None, 1 << 26, 8, 2, 0, P, P, P, P, None) == -2
+    assert "fewer than 2^26" in _said(lib)
+
+
+@pytest.mark.parametrize("E,M,N,K", [
+    (1, (1 << 30) - (1 << 17), 1, 1),    # row tiles of 64, 256 threads each
+    (1024, 8, 256, 1 << 20),             # the weights' gradient's tiles, in eights over the dies
+])
+def test_grouped_refuses_more_than_a_launch_holds(lib, E, M, N, K):
+    assert lib.bcjr_grouped_matmul(P, 1, K, M, None, P, K, 1, P, E, M, N, K, 0, P, None) == -2
+    assert "more tiles" in _said(lib)
+    assert lib.bcjr_grouped_wgrad(P, 1, N, P, K, M, None, P, E, M, N, K, 0, 1, P, None) == -2
+    assert "more tiles" in _said(lib)
+
+
 def test_route_workspace(lib):
     n = ctypes.c_size_t(7)
     assert lib.bcjr_moe_route_workspace(8, 64, ctypes.byref(n)) == 0 and n.value == 0
