@@ -25,10 +25,10 @@
 // stats[row] = (m, 1 / the sum, c, c - r / p_r; n as a double, 2 unused).
 //
 // Bound by the logits' bytes, at a copy's rate: 4,096 rows of 50,257 bfloat16, 64
-// entries, take 83 us (loss, 4.9 TB/s) and 173 (gradient, 4.75), together in one call
-// 210 (3.9 of one read and one write: part of a row is read twice, and neither the
-// loads nor the stores overlap the other half of the same row).  8,192 rows of
-// 131,072 take 389 (5.5), 845 (5.1) and 980 (4.4).
+// entries, take 83 us (loss, 4.9 TB/s) and 173 (gradient, 4.75), and in one call 210
+// (3.9: a row's loads wait for its stores to begin, and the rows beside it on a
+// compute unit cover only part of that).  8,192 rows of 131,072 take 389 (5.5), 845
+// (5.1) and 980 (5.5, with the half of a row that is not kept and read twice).
 #include "bcjr_moe_device.h"
 #include "bcjr_moe_kernels.h"
 
