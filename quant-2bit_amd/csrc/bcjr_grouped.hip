@@ -289,63 +289,48 @@ __device__ __forceinline__ void group_rows(const int32_t* offsets, int E, int M,
 // dies in turn, each with an L2 of its own, so each die takes a contiguous part
 // of the tiles, ordered by expert, then column, then row: an expert's weights
 // are read by one die (two at the seams), and neighbours share a column panel.
-// Tiles of full height come first, those with fewer rows after them, so that the
-// short ones fill the chip's last round.
+// (All tiles of full height before the short ones fill the last round better, but
+// read the weights twice: 64 uneven groups of 32,768 rows, 2048 x 2048, 351 us for
+// 336.  Parts by cost, a short tile half of a full one, 344; the search for them
+// takes longer, 276 for 262 with even groups.)
 template <int BM>
-__device__ __forceinline__ bool find_place(const int32_t* offsets, int E, int M, int nt, int64_t id, Place* out) {
+__device__ __forceinline__ bool find_place(const int32_t* offsets, int E, int M, int nt, int id, Place* out) {
   const int lane = threadIdx.x & 63;
-  int64_t full = 0, part = 0;
-  for (int i = 0; i <= E; i += 64) {
-    int a, b;
+  int a, b, n, upto;  // of this lane's group: rows, row tiles, row tiles up to its end
+  auto groups = [&](int i) {
     group_rows(offsets, E, M, i + lane, &a, &b);
-    int n = (b - a) / BM, m = (b - a) % BM != 0;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o);
-    full += n;
-    part += __popcll(__ballot(m));
-  }
-  full = uniform(full) * nt;
-  part = uniform(part) * nt;
-  const int die = (int)(id & 7);
-  const int64_t per_full = (full + 7) / 8, per_part = (part + 7) / 8;
-  int64_t seq = id >> 3;
-  // how many of each this die has
-  const int64_t f0 = min(die * per_full, full), f1 = min(f0 + per_full, full);
-  const int64_t p0 = min(die * per_part, part), p1 = min(p0 + per_part, part);
-  const bool is_full = seq < f1 - f0;
-  int64_t at;
-  if (is_full) {
-    at = f0 + seq;
-  } else {
-    at = p0 + seq - (f1 - f0);
-    if (at >= p1) return false;
-  }
-  int64_t done = 0;
-  for (int i = 0; i <= E; i += 64) {
-    int a, b;
-    group_rows(offsets, E, M, i + lane, &a, &b);
-    const int n = is_full ? (b - a) / BM : (b - a) % BM != 0;
-    int upto = n;
+    upto = n = (b - a + BM - 1) / BM;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(upto, o);
-      if (lane >= o) upto += y;
+      const int x = __shfl_up(upto, o);
+      if (lane >= o) upto += x;
     }
-    const int64_t first = (done + upto - n) * nt;
-    const unsigned long long here = __ballot(at >= first && at < first + (int64_t)n * nt);
+  };
+  int64_t total = 0;
+  for (int i = 0; i <= E; i += 64) {
+    groups(i);
+    total += uniform(__shfl(upto, 63));
+  }
+  if (total > (int64_t)M / BM + E + 1) return false;  // offsets that do not ascend
+  const int tiles = (int)total * nt, per = (tiles + 7) / 8, seq = id >> 3, at = (id & 7) * per + seq;
+  if (seq >= per || at >= tiles) return false;
+  int done = 0;
+  for (int i = 0; i <= E; i += 64) {
+    if (E >= 64) groups(i);
+    const int first = (done + upto - n) * nt;
+    const unsigned long long here = __ballot(at >= first && at < first + n * nt);
     if (here) {
       const int src = __ffsll(here) - 1;
       const int ea = uniform(__shfl(a, src)), eb = uniform(__shfl(b, src)), en = uniform(__shfl(n, src));
-      const int64_t f = uniform((done + __shfl(upto - n, src)) * nt);
-      const int local = uniform((int)(at - f));
-      out->e = uniform(i + src);
-      out->r0 = is_full ? ea + (int64_t)(local % en) * BM : ea + (int64_t)((eb - ea) / BM) * BM;
-      out->r1 = is_full ? out->r0 + BM : eb;
+      const int local = at - uniform(__shfl(first, src)), r0 = ea + local % en * BM;
+      out->e = i + src;
+      out->r0 = r0;
+      out->r1 = min(r0 + BM, eb);
       out->n0 = local / en;
-      out->first = out->r0 == ea;
+      out->first = r0 == ea;
       return true;
     }
-    done += __shfl(upto, 63);
+    done += uniform(__shfl(upto, 63));
   }
   return false;
 }
@@ -669,8 +654,7 @@ hipError_t launch_tile(const GroupedParams& P, hipStream_t stream) {
     }
     tiles = best * 8 * P.E;
   } else {
-    // full and short tiles are each shared by the dies in equal parts
-    tiles = (max_tiles(P.M, P.E, BM) * ((P.N + BN - 1) / BN) + 7) / 8 * 8 + 8;
+    tiles = (max_tiles(P.M, P.E, BM) * ((P.N + BN - 1) / BN) + 7) / 8 * 8;
   }
   if (tiles > INT32_MAX) return hipErrorInvalidConfiguration;
   void* args[] = {(void*)&Q};
