@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void wgrad_any_kernel(GroupedParams P) {
 // With many rows the matrix instructions bind, at the clock that the card's power
 // allows under them: 64 groups of 512 rows, 2048 x 2048, take 245 us forward, 1.12
 // PFLOP/s (a library's product of 8192 cubed 1.32), 1.75 GHz with the matrix units
-// busy 56 % of the time; uneven groups add short tiles and a longer last round (0.75).
+// busy 56 % of the time; uneven groups add short tiles and a longer last round (0.82).
 // The weights' gradient, 465 us, also writes E N K values in float32.  With few
 // rows the weights' bytes bind: 32 rows on about 26 of 64 experts take 45 us, 4.9 TB/s.
 // Side by side on the large products, 256 x 256 tiles beat 128 x 256 and 128 x 128
@@ -671,23 +671,35 @@ bool chunked(const void* p, int64_t ld, int64_t rows) {
 // Side of the square output tiles.  Larger tiles load less for the same work and
 // smaller ones leave fewer compute units idle; the counts below take every group
 // to have a short tile.  Measured (microseconds at 256 / 128 / 64, bfloat16, the
-// groups as a router with favourites fills them):
-//   products  4096 tokens x 8, 64 experts, 2048 x 2048 (1,536 tiles of 256)  351 / 399 / 620
-//             1024 x 8, 64, 2048 x 2048 (768)       166 / 181 / 220
-//             256 x 8, 64, 2048 x 2048 (576)        125 / 120 / 132
-//             2048 x 4, 64, 1024 x 1024 (384)        57 /  46 /  61
-//             1024 x 2, 8, 1024 x 1024 (192 of 128)  29 /  15 /  16
-//             256 x 2, 8, 512 x 512 (48 of 128)      16 / 8.6 / 6.4
+// groups as a router with favourites fills them; M rows, E experts, K -> N; tiles):
+//   products  32,768, 64, 2048 -> 2048 (1,536 of 256)   332 / 367 / 585
+//             32,768, 64, 1024 -> 1024 (768)             97 / 106 / 169
+//             16,384, 16, 2048 -> 2048 (640)            158 / 169 / 270
+//             16,384, 64, 2048 -> 1024 (512)            115 / 117 / 166
+//              8,192, 16, 2048 -> 2048 (384)            107 / 105 / 151
+//              8,192,  8, 2048 -> 2048 (320)            102 /  94 / 139
+//   and of groups that hardly fill a tile of 256:
+//             12,000, 64, 2048 -> 2048 (888)            178 / 189 / 247
+//              8,192, 64, 2048 -> 2048 (768)            169 / 163 / 196
+//              2,048, 64, 2048 -> 2048 (576)            126 / 118 / 124
+//              2,048,  8, 1024 -> 1024 (192 of 128)      29 /  15 /  15
+//                512,  8,  512 ->  512 (48 of 128)       16 / 8.1 / 5.9
 //   and of a few rows, where the weights' bytes count and not the row tiles:
-//             4 tokens x 8, 64, 2048 x 2048 (512 of 128)  51 / 46 / 44
-//             8 x 2, 8, 4096 x 4096 (256 of 128)          79 / 60 / 53
-//   weights' gradient  2048 x 2 on 8 experts, 2048 x 2048 (512)  56 / 57 / 92
-//             2048 x 2 on 16, 1024 x 1024 (256; 1,024 of 128)    50 / 26 / 38
-//             2048 on 4, 512 x 2048 (64; 256 of 128)             45 / 20 / 17
-int product_side(const GroupedParams& P) {
+//              1,024, 64, 1024 -> 2048 (1,152 of 128)    58 /  50 /  51
+//                512, 64, 2048 -> 2048 (1,088)          114 / 104 / 101
+//                256, 64, 2048 -> 2048 (1,056)          111 /  99 /  93
+//                 32, 64, 2048 -> 2048 (512)             52 /  45 /  44
+//                 16,  8, 4096 -> 4096 (256)             81 /  60 /  52
+//   the same by w (E, K, N), whose tiles of 64 are read in pieces of 128 bytes:
+//                512, 64, 2048 -> 1024 (576)              - /  42 /  49
+//   weights' gradient  4,096 rows, 8 experts, 2048 x 2048 (512)     55 / 55 / 91
+//              4,096, 16, 1024 x 1024 (256; 1,024 of 128)           49 / 25 / 38
+//              2,048, 4, 512 x 2048 (64; 256 of 128)                44 / 20 / 17
+int product_side(const GroupedParams& P, bool b_is_nk) {
   const int64_t groups = P.E < P.M ? P.E : P.M;
   auto tiles = [&](int64_t s) { return (P.M / s + groups) * ((P.N + s - 1) / s); };
-  if (tiles(256) >= 700) return 256;
+  if (P.M >= 160 * groups && tiles(256) >= 500) return 256;
+  if (P.M <= 12 * groups && b_is_nk) return 64;
   return tiles(128) < (P.M <= 64 * groups ? 512 : 176) ? 64 : 128;
 }
 int wgrad_side(const GroupedParams& P) {
@@ -697,7 +709,7 @@ int wgrad_side(const GroupedParams& P) {
 
 template <class E, int MODE, class O>
 hipError_t launch_side(const GroupedParams& P, hipStream_t stream) {
-  const int side = MODE == GM_WG ? wgrad_side(P) : product_side(P);
+  const int side = MODE == GM_WG ? wgrad_side(P) : product_side(P, MODE != GM_KN);
   return side == 256   ? launch_tile<E, O, MODE, 256, 256>(P, stream)
          : side == 128 ? launch_tile<E, O, MODE, 128, 128>(P, stream)
                        : launch_tile<E, O, MODE, 64, 64>(P, stream);
