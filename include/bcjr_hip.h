@@ -308,7 +308,8 @@ int bcjr_moe_route_backward(const void* logits, int dtype, int64_t ld, const uin
  * `a` (a_rows rows, row stride lda elements; a place outside [0, a_rows) is a
  * zero row), or row p where rows is NULL.  Places [offsets[e], offsets[e+1])
  * belong to expert e (offsets (E+1) on the device, ascending, offsets[0] taken as
- * 0 and all clamped to [0, M]); the places behind offsets[E] get zeros.
+ * 0 and all clamped to [0, M]; where they do not ascend, out may stay as it is);
+ * the places behind offsets[E] get zeros.
  *   b_is_nk = 1: b (E, N, K), out = a b^T (weights as a linear layer holds them)
  *   b_is_nk = 0: b (E, K, N), out = a b
  * with row stride ldb, the matrices of b back to back.

@@ -288,6 +288,35 @@ def test_gathered_rows(bcjr_mod, T, E, k, N, K, dtype):
     assert (y[live_rows:] == 0).all()
 
 
+@pytest.mark.parametrize("N,K,style", [(1032, 1160, "skew"), (1160, 1032, "even"), (1033, 1161, "short")])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_grouped_many_rows(bcjr_mod, N, K, style, dtype):
+    """Rows and tiles enough for the largest tiles, forward and backward."""
+    test_grouped_forward_backward(bcjr_mod, 20000, 40, N, K, style, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gathered_many_rows(bcjr_mod, dtype):
+    test_gathered_rows(bcjr_mod, 5000, 40, 4, 1032, 1160, dtype)
+
+
+@pytest.mark.parametrize("M,N,K", [(60, 700, 1600), (200, 1600, 700), (1500, 1600, 700), (4000, 1600, 1700)])
+def test_grouped_same_bits_beside_other_sizes(bcjr_mod, M, N, K):
+    """A row's product does not depend on how many rows its call has, nor on the tiles that it is cut into."""
+    g = gen(M)
+    E = 20
+    x = torch.randn(M, K, device=DEV, generator=g).bfloat16()
+    w = torch.randn(E, N, K, device=DEV, generator=g).bfloat16()
+    gc = torch.Generator()
+    gc.manual_seed(M)
+    off = groups_of(M, E, "even", gc)
+    y = bcjr_mod.grouped_matmul(x, w, off)
+    e = E // 2
+    a, b = int(off[e]), int(off[e + 1])
+    alone = bcjr_mod.grouped_matmul(x[a:b], w[e:e + 1], torch.tensor([0, b - a], dtype=torch.int32, device=DEV))
+    assert torch.equal(alone, y[a:b])
+
+
 def test_places_without_expert_do_not_leak(bcjr_mod):
     """NaN in rows behind the last group reach neither y nor the gradients."""
     M, E, N, K = 200, 4, 96, 160
