@@ -692,7 +692,10 @@ bool chunked(const void* p, int64_t ld, int64_t rows) {
 //                 16,  8, 4096 -> 4096 (256)             81 /  60 /  52
 //   the same by w (E, K, N), whose tiles of 64 are read in pieces of 128 bytes:
 //                512, 64, 2048 -> 1024 (576)              - /  42 /  49
-//   weights' gradient  4,096 rows, 8 experts, 2048 x 2048 (512)     55 / 55 / 91
+//   weights' gradient  32,768 rows, 64 experts, 2048 x 2048 (4,096) 468 / 564 / 985
+//              8,192, 16, 2048 x 2048 (1,024)                      129 / 130 / 205
+//              16,384, 8, 2048 x 2048 (512)                        179 / 168 / 273
+//              4,096, 8, 2048 x 2048 (512)                          55 / 55 / 91
 //              4,096, 16, 1024 x 1024 (256; 1,024 of 128)           49 / 25 / 38
 //              2,048, 4, 512 x 2048 (64; 256 of 128)                44 / 20 / 17
 int product_side(const GroupedParams& P, bool b_is_nk) {
@@ -704,7 +707,7 @@ int product_side(const GroupedParams& P, bool b_is_nk) {
 }
 int wgrad_side(const GroupedParams& P) {
   auto tiles = [&](int64_t s) { return P.E * ((P.N + s - 1) / s) * ((P.K + s - 1) / s); };
-  return tiles(256) >= 384 ? 256 : tiles(128) >= 400 ? 128 : 64;
+  return tiles(256) >= 640 ? 256 : tiles(128) >= 400 ? 128 : 64;
 }
 
 template <class E, int MODE, class O>
