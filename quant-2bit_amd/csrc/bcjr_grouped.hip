@@ -620,7 +620,14 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
         struct alignas(4 * sizeof(typename O::raw)) { typename O::raw v[4]; } o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o.v[e] = O::put(v[e]);
-        if (m < mend && n < nend) *(decltype(o)*)(out + m * nend + n) = o;
+        if (m < mend && n < nend) {
+          if constexpr (MODE == GM_WG) {  // past the caches, which hold the rows (1,024 x 8 rows: 272 -> 236 us)
+            typedef uint32_t vec_t __attribute__((ext_vector_type(sizeof(o) / 4)));
+            __builtin_nontemporal_store(__builtin_bit_cast(vec_t, o), (vec_t*)(out + m * nend + n));
+          } else {
+            *(decltype(o)*)(out + m * nend + n) = o;
+          }
+        }
       }
     } else {
       constexpr int lanes = WC < 64 ? WC : 64, rows = 64 / lanes;
