@@ -25,10 +25,10 @@
 // stats[row] = (m, 1 / the sum, c, c - r / p_r; n as a double, 2 unused).
 //
 // Bound by the logits' bytes, at a copy's rate: 4,096 rows of 50,257 bfloat16, 64
-// entries, take 83 us (loss, 4.9 TB/s) and 173 (gradient, 4.75), and in one call 210
-// (3.9: a row's loads wait for its stores to begin, and the rows beside it on a
-// compute unit cover only part of that).  8,192 rows of 131,072 take 389 (5.5), 845
-// (5.1) and 980 (5.5, with the half of a row that is not kept and read twice).
+// entries, take 83 us (loss, 4.9 TB/s) and 166 (gradient, 4.95), and in one call 197
+// (4.2: a row's loads wait for its stores to begin, and the rows beside it on a
+// compute unit cover only part of that).  8,192 rows of 131,072 take 389 (5.5), 785
+// (5.5) and 915 (5.9, with the half of a row that is not kept and read twice).
 #include "bcjr_moe_device.h"
 #include "bcjr_moe_kernels.h"
 
@@ -70,7 +70,8 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
-template <class E, int KIND, bool VEC, int NT, int C>
+// PAST: the gradient is stored past the caches.
+template <class E, int KIND, bool VEC, int NT, int C, bool PAST = false>
 __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParams P) {
   constexpr int N = VEC ? Vec16<E>::N : 1, NW = NT / 64;
   using raw = typename E::raw;
@@ -278,7 +279,11 @@ __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParam
       unpack16<E>(t, z);
 #pragma unroll
       for (int i = 0; i < N; ++i) z[i] = out(z[i]);
-      *(u32x4*)(g - lead + (int64_t)v * N) = pack16<E>(z);
+      u32x4* to = (u32x4*)(g - lead + (int64_t)v * N);
+      if constexpr (PAST)
+        __builtin_nontemporal_store(pack16<E>(z), to);
+      else
+        *to = pack16<E>(z);
     };
     int v = v0 + tid;
     if constexpr (VEC) {
@@ -332,36 +337,43 @@ __global__ __launch_bounds__(NT, C > 8 ? 4 : 8) void distill_kernel(DistillParam
 //   4,096 rows of 50,257 bfloat16 (6,282)           217 /  207 /  255
 //   8,192 rows of 131,072 bfloat16 (16,384)       1,215 /  986 / 1,076
 //   4,096 rows of 131,072 float32 (32,768)        1,212 / 1,112 /  920
-// (Keeping none cost 140, 34, 14, 218, 1,055 and 1,166 at the best width of each.)
+// (Keeping none cost 140, 34, 14, 218, 1,055 and 1,166 at the best width of each.  All
+// stored through the caches; large gradients go past them now, 197 and 915 for 207 and
+// 986.)
 int row_threads(int64_t nvec) { return nvec < 3000 ? 256 : nvec <= 16384 ? 512 : 1024; }
 
-template <class E>
+template <class E, bool PAST>
 const void* distill_ptr(int kind, bool vec, int nt) {
   if (kind == DISTILL_BACKWARD)
-    return vec ? (const void*)distill_kernel<E, DISTILL_BACKWARD, true, 1024, 0>
+    return vec ? (const void*)distill_kernel<E, DISTILL_BACKWARD, true, 1024, 0, PAST>
                : (const void*)distill_kernel<E, DISTILL_BACKWARD, false, 1024, 0>;
   if (kind == DISTILL_LOSS)
     return nt == 256   ? (const void*)distill_kernel<E, DISTILL_LOSS, true, 256, 0>
            : nt == 512 ? (const void*)distill_kernel<E, DISTILL_LOSS, true, 512, 0>
                        : (const void*)distill_kernel<E, DISTILL_LOSS, true, 1024, 0>;
   if (!vec) return (const void*)distill_kernel<E, DISTILL_BOTH, false, 1024, 0>;
-  return nt == 256   ? (const void*)distill_kernel<E, DISTILL_BOTH, true, 256, 12>
-         : nt == 512 ? (const void*)distill_kernel<E, DISTILL_BOTH, true, 512, 16>
-                     : (const void*)distill_kernel<E, DISTILL_BOTH, true, 1024, 16>;
+  return nt == 256   ? (const void*)distill_kernel<E, DISTILL_BOTH, true, 256, 12, PAST>
+         : nt == 512 ? (const void*)distill_kernel<E, DISTILL_BOTH, true, 512, 16, PAST>
+                     : (const void*)distill_kernel<E, DISTILL_BOTH, true, 1024, 16, PAST>;
+}
+template <class E>
+const void* distill_ptr(int kind, bool vec, int nt, bool past) {
+  return past ? distill_ptr<E, true>(kind, vec, nt) : distill_ptr<E, false>(kind, vec, nt);
 }
 
 }  // namespace
 
 hipError_t launch_distill(const DistillParams& P, int dtype, int kind, hipStream_t stream) {
   const size_t es = dtype == 0 ? 4 : 2;
+  const bool past = P.T * P.V * (int64_t)es > kPastCaches;
   // 16-byte loads and stores need input and output rows in step
   const bool vec = kind == DISTILL_LOSS ||
                    (((reinterpret_cast<uintptr_t>(P.logits) ^ reinterpret_cast<uintptr_t>(P.grad)) & 15) == 0 &&
                     (P.T == 1 || (P.ld - P.V) * (int64_t)es % 16 == 0));
   const int nt = kind == DISTILL_BACKWARD || !vec ? 1024 : row_threads((int64_t)P.V * (int64_t)es / 16);
-  const void* fn = dtype == 0   ? distill_ptr<F32>(kind, vec, nt)
-                   : dtype == 1 ? distill_ptr<BF16>(kind, vec, nt)
-                                : distill_ptr<F16>(kind, vec, nt);
+  const void* fn = dtype == 0   ? distill_ptr<F32>(kind, vec, nt, past)
+                   : dtype == 1 ? distill_ptr<BF16>(kind, vec, nt, past)
+                                : distill_ptr<F16>(kind, vec, nt, past);
   const size_t lds = kind == DISTILL_LOSS && !P.teacher_lse ? 0 : ((size_t)P.V + 8 + 31) / 32 * 4 + 16;
   hipError_t e = hipSuccess;
   if (lds > 60000) e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

@@ -621,9 +621,9 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
 #pragma unroll
         for (int e = 0; e < 4; ++e) o.v[e] = O::put(v[e]);
         if (m < mend && n < nend) {
-          if constexpr (MODE == GM_WG) {  // past the caches, which hold the rows (1,024 x 8 rows: 272 -> 236 us)
+          if (MODE == GM_WG && P.past) {
             typedef uint32_t vec_t __attribute__((ext_vector_type(sizeof(o) / 4)));
-            __builtin_nontemporal_store(__builtin_bit_cast(vec_t, o), (vec_t*)(out + m * nend + n));
+            store_past((vec_t*)(out + m * nend + n), __builtin_bit_cast(vec_t, o));
           } else {
             *(decltype(o)*)(out + m * nend + n) = o;
           }
@@ -660,6 +660,7 @@ hipError_t launch_tile(const GroupedParams& P, hipStream_t stream) {
       if (per < best) best = per, Q.split = xa;
     }
     tiles = best * 8 * P.E;
+    Q.past = (int64_t)P.E * P.N * P.K * (int64_t)sizeof(typename O::raw) > kPastCaches;
   } else {
     tiles = (max_tiles(P.M, P.E, BM) * ((P.N + BN - 1) / BN) + 7) / 8 * 8;
   }

@@ -100,4 +100,13 @@ __device__ __forceinline__ float group_max(float x, float* part) {
   return s;
 }
 
+// Stores v past the caches.  (Between the two, the compiler would join it with a
+// plain store of the same in another branch.)
+template <class V>
+__device__ __forceinline__ void store_past(V* to, V v) {
+  asm volatile("" ::: "memory");
+  __builtin_nontemporal_store(v, to);
+  asm volatile("" ::: "memory");
+}
+
 }  // namespace bcjr

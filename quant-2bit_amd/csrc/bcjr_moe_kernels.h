@@ -85,7 +85,10 @@ struct GroupedParams {
   // null, gets the rounded weights of the experts that have rows
   bool b_f32;
   void* b_copy;
-  int split;  // set by the launch
+  // set by the launch: dies across the rows of the weights' gradient, and whether it
+  // is stored past the caches
+  int split;
+  bool past;
 };
 
 struct DistillParams {
@@ -102,6 +105,14 @@ struct DistillParams {
   double inv_tau;
   float scale_hi, scale_lo;  // log2(e) / tau in two parts, the second above 0
 };
+
+// Gradients of more bytes than the last-level cache holds are stored past the caches,
+// which keep what is read instead; smaller ones are found there by their reader.
+// (Microseconds, cached / past.  Distillation's loss and gradient and a copy of the
+// gradient: 1,024 x 32,000 bfloat16, 66 MB, 55 / 59; 4,096 x 32,000, 262 MB, 238 / 241;
+// 4,096 x 50,257, 412 MB, 360 / 357; without the copy 8,192 x 131,072, 2.1 GB, 976 / 911 (gradient alone 845 / 785).
+// Weights' gradient of 64 experts, 2048 x 2048 float32, 1.07 GB, 8,192 rows: 272 / 236.)
+constexpr int64_t kPastCaches = 300 << 20;
 
 // Stores `text` for bcjr_last_error() and returns the status (bcjr_capi.hip).
 int report_failure(int status, const char* text);
