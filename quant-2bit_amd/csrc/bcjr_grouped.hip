@@ -519,8 +519,8 @@ __global__ __launch_bounds__(kFastThreads, 2) void grouped_tile_kernel(GroupedPa
   // float32 weights go through registers: a step's 16-byte loads, 16 lanes a row,
   // wait in `wide` for the next step, and are rounded on their way into LDS.  The
   // first row tile of a group also leaves the rounded weights behind, if asked.
-  // (32,768 rows, 64 experts, 2048 x 2048: 496 us, with the copy 598; a copy first
-  // and then the product 274 + 343.  32 rows: 56, with the copy 119; 272 + 26.)
+  // (32,768 rows, 64 experts, 2048 x 2048: 453 us, with the copy 553; a copy first
+  // and then the product 343 + 336.  32 rows: 61, with the copy 124; 272 + 42.)
   constexpr int SW = BF32 ? 2 * SB : 1;
   u32x4 wide[SW];
   const int wr = tid >> 4, wc = (tid & 15) * 4;  // row (32 more for each load), column
